@@ -1,0 +1,235 @@
+// Writing tokens into the 4-bit key/value cache, and reading rows of it back.
+//
+// Both are one pass over the data: a thread has 8 channels of one row, the
+// four threads of a quad one channel group, so the group's minimum and
+// maximum are two DPP exchanges and no data moves through LDS.  Each thread
+// takes the key row and the value row of its token (two independent loads in
+// flight).
+#include <type_traits>
+
+#include "asa_cache.hpp"
+#include "asa_device.hpp"
+
+namespace asa {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Values at or past this bound are taken as the bound (NaN as 0), so that a
+// group's range and scale are finite.
+constexpr float kMostCached = 0x1p126f;
+
+// 8 consecutive channels from `src` as floats; channels at or past `nv` give 0.
+template <typename T, bool CHUNKS>
+__device__ __forceinline__ void load8(const T* src, int nv, float* x) {
+  if constexpr (CHUNKS) {
+    if constexpr (std::is_same<T, float>::value) {
+      const float4 a = *reinterpret_cast<const float4*>(src);
+      const float4 b = *reinterpret_cast<const float4*>(src + 4);
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+      x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(src);
+      T e[8];
+      __builtin_memcpy(e, &u, 16);
+      for (int j = 0; j < 8; ++j) x[j] = Elem<T>::load(e + j);
+    }
+  } else {
+    for (int j = 0; j < 8; ++j) x[j] = j < nv ? Elem<T>::load(src + j) : 0.0f;
+  }
+}
+
+template <typename T, bool CHUNKS>
+__device__ __forceinline__ void store8(T* dst, int nv, const float* x) {
+  if constexpr (CHUNKS) {
+    if constexpr (std::is_same<T, float>::value) {
+      *reinterpret_cast<float4*>(dst) = float4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<float4*>(dst + 4) = float4{x[4], x[5], x[6], x[7]};
+    } else {
+      T e[8];
+      for (int j = 0; j < 8; ++j) Elem<T>::store(e + j, x[j]);
+      uint4 u;
+      __builtin_memcpy(&u, e, 16);
+      *reinterpret_cast<uint4*>(dst) = u;
+    }
+  } else {
+    for (int j = 0; j < 8; ++j)
+      if (j < nv) Elem<T>::store(dst + j, x[j]);
+  }
+}
+
+// The exact value of a - b as an unevaluated sum hi + lo.
+__device__ __forceinline__ void two_diff(float a, float b, float& hi, float& lo) {
+  hi = a - b;
+  const float t = hi - a;
+  lo = (a - (hi - t)) - (b + t);
+}
+
+// The codes (nibble j: channel j) and the group's params of 8 channels x, of
+// which nv belong to the row.  Called by whole quads: a quad is a group.
+__device__ __forceinline__ uint32_t quantise8(float* x, int nv, uint32_t& params) {
+  bool wild = false;
+  for (int j = 0; j < 8; ++j) wild |= !(fabsf(x[j]) <= kMostCached);
+  if (wild)
+    for (int j = 0; j < 8; ++j)
+      x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -kMostCached), kMostCached) : 0.0f;
+  float lo = __builtin_inff(), hi = -__builtin_inff();
+  for (int j = 0; j < 8; ++j)
+    if (j < nv) {
+      lo = fminf(lo, x[j]);
+      hi = fmaxf(hi, x[j]);
+    }
+  lo = fminf(lo, __uint_as_float(lane_xor<1>(__float_as_uint(lo))));
+  hi = fmaxf(hi, __uint_as_float(lane_xor<1>(__float_as_uint(hi))));
+  lo = fminf(lo, __uint_as_float(lane_xor<2>(__float_as_uint(lo))));
+  hi = fmaxf(hi, __uint_as_float(lane_xor<2>(__float_as_uint(hi))));
+  // m: towards zero in the bits, one step further down for a cut negative
+  const uint32_t lb = __float_as_uint(lo);
+  const uint32_t mb = (lb & 0xffff0000u) + (lo < 0.0f && (lb & 0xffffu) ? 0x10000u : 0u);
+  const float m = __uint_as_float(mb);
+  // s: 15 s has 12 significant bits, so the comparison with the exact
+  // max - m = d + dl is exact; the estimate is at most two steps low
+  float d, dl;
+  two_diff(hi, m, d, dl);
+  uint32_t sb = 0u;
+  if (d > 0.0f) {
+    sb = __float_as_uint(fmaxf(d * (1.0f / 15.0f), 0x1p-126f)) & 0xffff0000u;
+    for (int i = 0; i < 2; ++i) {
+      const float t = 15.0f * __uint_as_float(sb);
+      if (t < d || (t == d && dl > 0.0f)) sb += 0x10000u;
+    }
+  }
+  const float s = __uint_as_float(sb);
+  params = (sb >> 16) | mb;
+  // c: y is near (x - m) / s, so one of the borders on either side of
+  // floor(y) + 1/2 is the only one in doubt, and an exact comparison with it
+  // settles the code whatever y was rounded to.
+  const float r = sb ? __builtin_amdgcn_rcpf(s) : 0.0f;
+  const float nm = -m * r;
+  uint32_t w = 0u;
+  // m + (k + 1/2) s: m is a multiple of 2^-7 of its power of two and the rest
+  // of 2^-8 of s's, so between |m| = 2^-8 s and 2^12 s the sum spans at most
+  // 22 bits and the fused product rounds nothing.
+  const float am = fabsf(m);
+  if (am == 0.0f || (am >= 0x1p-8f * s && am <= 0x1p12f * s)) {
+    for (int j = 7; j >= 0; --j) {
+      const float k = floorf(fmaf(x[j], r, nm));
+      const float border = fmaf(k + 0.5f, s, m);
+      const int c = int(k) + (x[j] > border ? 1 : 0);
+      w = (w << 4) | uint32_t(c);
+    }
+  } else {
+    for (int j = 7; j >= 0; --j) {
+      float t, tl;
+      two_diff(x[j], m, t, tl);
+      const float k = fminf(fmaxf(floorf(t * r), 0.0f), 15.0f);
+      const float border = (k + 0.5f) * s;
+      const int c = int(k) + (t > border || (t == border && tl > 0.0f) ? 1 : 0);
+      w = (w << 4) | uint32_t(c > 15 ? 15 : c);
+    }
+  }
+  if (nv < 8) w = nv <= 0 ? 0u : w & (0xffffffffu >> (4 * (8 - nv)));
+  return w;
+}
+
+template <typename T, bool CHUNKS>
+__global__ __launch_bounds__(kThreads) void cache_write_kernel(CacheRowsParams p, int lanes_shift, int nblk) {
+  const int bh = blockIdx.x / nblk, b = bh / p.c.heads, h = bh % p.c.heads;
+  const int t = (blockIdx.x - bh * nblk) * kThreads + threadIdx.x;
+  const int i = t >> lanes_shift, l = t & ((1 << lanes_shift) - 1);
+  const int g = l >> 2, o = l & 3;
+  const int count = p.limit ? min(p.limit[b], p.n) : p.n;
+  if (i >= count || g >= p.c.G) return;  // whole quads leave together
+  const int64_t pos = int64_t(p.start ? p.start[b] : 0) + i;
+  if (pos < 0 || pos >= (int64_t(1) << 31)) return;
+  const int64_t row = cache_row(p.c, p.table + size_t(b) * p.cols, p.cols, int(pos), h);
+  if (row < 0) return;
+  const int ch = 32 * g + 8 * o, nv = p.c.hd - ch;
+  const T* k = static_cast<const T*>(p.k) + size_t(b) * p.lk.sb + size_t(h) * p.lk.sh + size_t(i) * p.lk.sn + ch;
+  const T* v = static_cast<const T*>(p.v) + size_t(b) * p.lv.sb + size_t(h) * p.lv.sh + size_t(i) * p.lv.sn + ch;
+  float xk[8] = {}, xv[8] = {};
+  if (nv > 0) {  // rows that end inside the group: its last octets have no channels
+    load8<T, CHUNKS>(k, nv, xk);
+    load8<T, CHUNKS>(v, nv, xv);
+  }
+  uint32_t pk, pv;
+  const uint32_t wk = quantise8(xk, nv, pk);
+  const uint32_t wv = quantise8(xv, nv, pv);
+  const int G = p.c.G;
+  reinterpret_cast<uint32_t*>(p.c.k_codes)[row * (4 * G) + G * o + g] = wk;
+  reinterpret_cast<uint32_t*>(p.c.v_codes)[row * (4 * G) + 4 * g + o] = wv;
+  if (o == 0) {
+    p.c.k_params[row * G + g] = pk;
+    p.c.v_params[row * G + g] = pv;
+  }
+}
+
+// m + c s, rounded once: c s has 12 bits, the fused sum one rounding.
+__device__ __forceinline__ void values8(uint32_t w, uint32_t params, float* x) {
+  const float s = __uint_as_float(params << 16), m = __uint_as_float(params & 0xffff0000u);
+  for (int j = 0; j < 8; ++j) x[j] = fmaf(float((w >> (4 * j)) & 15u), s, m);
+}
+
+template <typename T, bool CHUNKS>
+__global__ __launch_bounds__(kThreads) void cache_read_kernel(CacheRowsParams p, int lanes_shift, int nblk) {
+  const int bh = blockIdx.x / nblk, b = bh / p.c.heads, h = bh % p.c.heads;
+  const int t = (blockIdx.x - bh * nblk) * kThreads + threadIdx.x;
+  const int i = t >> lanes_shift, l = t & ((1 << lanes_shift) - 1);
+  const int g = l >> 2, o = l & 3;
+  if (i >= p.n || g >= p.c.G) return;
+  const int ch = 32 * g + 8 * o, nv = p.c.hd - ch;
+  if (nv <= 0) return;
+  const int64_t pos = int64_t(p.start ? p.start[b] : 0) + i;
+  const int G = p.c.G;
+  int64_t row = -1;
+  if (pos >= 0 && pos < p.limit[b])
+    row = cache_row(p.c, p.table + size_t(b) * p.cols, p.cols, int(pos), h);
+  float xk[8] = {}, xv[8] = {};
+  if (row >= 0) {
+    const uint32_t wk = reinterpret_cast<const uint32_t*>(p.c.k_codes)[row * (4 * G) + G * o + g];
+    const uint32_t wv = reinterpret_cast<const uint32_t*>(p.c.v_codes)[row * (4 * G) + 4 * g + o];
+    const uint32_t pk = p.c.k_params[row * G + g], pv = p.c.v_params[row * G + g];
+    values8(wk, pk, xk);
+    values8(wv, pv, xv);
+  }
+  const size_t at = (size_t(bh) * p.n + i) * p.c.hd + ch;
+  store8<T, CHUNKS>(static_cast<T*>(p.ok) + at, nv, xk);
+  store8<T, CHUNKS>(static_cast<T*>(p.ov) + at, nv, xv);
+}
+
+// Threads of a row: 4 per channel group, rounded up to a power of two.
+int lanes_shift_of(int G) { return G > 2 ? 4 : G > 1 ? 3 : 2; }
+
+template <typename T>
+hipError_t launch_rows(const CacheRowsParams& p, bool write, hipStream_t s) {
+  const int sh = lanes_shift_of(p.c.G);
+  const long long threads = (long long)p.n << sh;
+  const long long nblk = (threads + kThreads - 1) / kThreads;
+  const long long blocks = nblk * p.B * p.c.heads;
+  if (threads >= (1LL << 31) || blocks >= (1LL << 31)) return hipErrorInvalidConfiguration;
+  const dim3 grid{unsigned(blocks)};
+  if (write) {
+    if (p.chunks) hipLaunchKernelGGL((cache_write_kernel<T, true>), grid, dim3(kThreads), 0, s, p, sh, int(nblk));
+    else hipLaunchKernelGGL((cache_write_kernel<T, false>), grid, dim3(kThreads), 0, s, p, sh, int(nblk));
+  } else {
+    if (p.chunks) hipLaunchKernelGGL((cache_read_kernel<T, true>), grid, dim3(kThreads), 0, s, p, sh, int(nblk));
+    else hipLaunchKernelGGL((cache_read_kernel<T, false>), grid, dim3(kThreads), 0, s, p, sh, int(nblk));
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_cache_write(const CacheRowsParams& p, int dtype, hipStream_t s) {
+  if (dtype == kElemBF16) return launch_rows<u16>(p, true, s);
+  if (dtype == kElemF16) return launch_rows<h16>(p, true, s);
+  return launch_rows<float>(p, true, s);
+}
+
+hipError_t launch_cache_read(const CacheRowsParams& p, int dtype, hipStream_t s) {
+  if (dtype == kElemBF16) return launch_rows<u16>(p, false, s);
+  if (dtype == kElemF16) return launch_rows<h16>(p, false, s);
+  return launch_rows<float>(p, false, s);
+}
+
+}  // namespace asa

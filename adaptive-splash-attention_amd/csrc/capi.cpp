@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/adasplash.h"
+#include "asa_cache.hpp"
 #include "asa_launch.hpp"
 
 static_assert(int(ASA_DTYPE_F32) == asa::kElemF32 && int(ASA_DTYPE_BF16) == asa::kElemBF16 &&
@@ -299,6 +300,143 @@ int select_plan_of(const Shape& s, bool from_scores, asa::SelectPlan* plan) {
   if (plan->cap < 0)
     return fail(ASA_ERR_UNSUPPORTED, "k_keep %d needs %zu bytes of LDS per block, device has %d",
                 s.k, plan->needs, max_lds);
+  return ASA_OK;
+}
+
+// ---------------------------------------------------------------------------
+// The 4-bit cache
+// ---------------------------------------------------------------------------
+constexpr int kMaxCacheQueries = 64;
+
+int validate_cache(const asa_cache* c, bool pointers, asa::CachePool* pool) {
+  if (!c) return fail(ASA_ERR_INVALID_ARGUMENT, "cache descriptor is NULL");
+  if (c->pages < 1 || c->kv_heads < 1)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "pages (%d) and kv_heads (%d) must be >= 1", c->pages,
+                c->kv_heads);
+  int shift = 4;
+  while (shift < 8 && (1 << shift) != c->page_size) ++shift;
+  if ((1 << shift) != c->page_size)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "page_size %d must be 16, 32, 64, 128 or 256",
+                c->page_size);
+  if (c->head_dim > 128)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "Head dimension too large (%d > 128)", c->head_dim);
+  if (c->head_dim < 1)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "head_dim %d must be >= 1", c->head_dim);
+  if ((long long)c->pages * c->kv_heads > (1LL << 40) / c->page_size)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "cache too large");
+  if (pointers) {
+    if (!c->k_codes || !c->v_codes || !c->k_params || !c->v_params)
+      return fail(ASA_ERR_INVALID_ARGUMENT, "a cache tensor is NULL");
+    if (int rc = check_aligned({c->k_codes, c->v_codes, c->k_params, c->v_params})) return rc;
+  }
+  *pool = asa::CachePool{c->pages, c->kv_heads, c->page_size, shift, c->head_dim,
+                         (c->head_dim + 31) / 32, static_cast<uint8_t*>(c->k_codes),
+                         static_cast<uint8_t*>(c->v_codes), static_cast<uint32_t*>(c->k_params),
+                         static_cast<uint32_t*>(c->v_params)};
+  return ASA_OK;
+}
+
+// Element strides {batch, head, row} of a cache call's operand.
+int cache_strides(const int64_t* st, int heads, int n, int hd, const char* name, asa::Lay* lay) {
+  if (st[0] == 0 && st[1] == 0 && st[2] == 0) {
+    *lay = contiguous(heads, n, hd);
+    return ASA_OK;
+  }
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0)
+      return fail(ASA_ERR_INVALID_ARGUMENT, "%s_strides[%d] = %lld must be >= 0", name, i,
+                  (long long)st[i]);
+  *lay = asa::Lay{st[0], st[1], st[2]};
+  return ASA_OK;
+}
+
+// Whether every row of an operand is a whole number of 16-byte chunks that
+// starts on one (then the kernels load and store chunks).
+bool whole_chunks(const void* p, const asa::Lay& l, int hd, int dtype) {
+  const int es = asa::elem_bytes(dtype);
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && hd % 8 == 0 && l.sb * es % 16 == 0 &&
+         l.sh * es % 16 == 0 && l.sn * es % 16 == 0;
+}
+
+int check_dtype(int dtype) {
+  if (dtype != ASA_DTYPE_F32 && dtype != ASA_DTYPE_BF16 && dtype != ASA_DTYPE_F16)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  return ASA_OK;
+}
+
+int validate_tokens(const asa_cache* c, const asa_cache_tokens* t, asa::CacheRowsParams* rp) {
+  if (int rc = validate_cache(c, true, &rp->c)) return rc;
+  if (!t) return fail(ASA_ERR_INVALID_ARGUMENT, "token descriptor is NULL");
+  if (t->batch < 1 || t->n < 1 || t->max_pages < 1)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "batch (%d), n (%d) and max_pages (%d) must be >= 1",
+                t->batch, t->n, t->max_pages);
+  if (int rc = check_dtype(t->dtype)) return rc;
+  if (!t->page_table) return fail(ASA_ERR_INVALID_ARGUMENT, "page_table is NULL");
+  // 16 threads per row at most, 256 to a block
+  const long long blocks = ((long long)t->n * 16 + 255) / 256;
+  if (t->n >= (1 << 26) || (long long)t->batch * c->kv_heads > ((1LL << 31) - 1) / blocks)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "too many tokens in one call");
+  rp->B = t->batch;
+  rp->n = t->n;
+  rp->cols = t->max_pages;
+  rp->table = t->page_table;
+  rp->start = t->start;
+  return ASA_OK;
+}
+
+int validate_query(const asa_cache* c, const asa_cache_query* a, bool pointers,
+                   asa::CacheAttnParams* ap) {
+  if (int rc = validate_cache(c, pointers, &ap->c)) return rc;
+  if (!a) return fail(ASA_ERR_INVALID_ARGUMENT, "query descriptor is NULL");
+  if (a->batch < 1 || a->heads < 1 || a->max_pages < 1)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "batch (%d), heads (%d) and max_pages (%d) must be >= 1",
+                a->batch, a->heads, a->max_pages);
+  if (a->nq < 1 || a->nq > kMaxCacheQueries)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "nq %d out of range [1, %d]", a->nq, kMaxCacheQueries);
+  if (a->heads % c->kv_heads)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "heads (%d) must be a multiple of kv_heads (%d)",
+                a->heads, c->kv_heads);
+  if (int rc = check_dtype(a->dtype)) return rc;
+  if (!std::isfinite(a->alpha)) return fail(ASA_ERR_INVALID_ARGUMENT, "alpha is not finite");
+  if (!std::isfinite(a->sm_scale)) return fail(ASA_ERR_INVALID_ARGUMENT, "sm_scale is not finite");
+  if (a->max_length < 0)
+    return fail(ASA_ERR_INVALID_ARGUMENT, "max_length %d must be >= 0", a->max_length);
+  long long most = (long long)a->max_pages * c->page_size;
+  if (a->max_length > 0 && a->max_length < most) most = a->max_length;
+  if (most >= (1 << 28))
+    return fail(ASA_ERR_INVALID_ARGUMENT, "max_length (%lld) must be below 2^28", most);
+  const long long rows = (long long)a->batch * a->heads * a->nq;
+  if (rows >= (1LL << 24)) return fail(ASA_ERR_INVALID_ARGUMENT, "too many query rows (%lld)", rows);
+  if (pointers && (!a->page_table || !a->lengths))
+    return fail(ASA_ERR_INVALID_ARGUMENT, "page_table or lengths is NULL");
+  ap->B = a->batch;
+  ap->H = a->heads;
+  ap->NQ = a->nq;
+  ap->cols = a->max_pages;
+  ap->maxlen = int(most);
+  ap->rep = a->heads / c->kv_heads;
+  ap->R = ap->rep * a->nq;
+  ap->table = a->page_table;
+  ap->lengths = a->lengths;
+  ap->q_idx = a->q_idx;
+  ap->alpha = std::fmax(1.05f, std::fmin(a->alpha, 3.0f));
+  ap->scale = a->sm_scale;
+  return cache_strides(a->q_strides, a->heads, a->nq, c->head_dim, "q", &ap->lq);
+}
+
+// Chooses how the call runs on the current device; its workspace bytes.
+int plan_query(asa::CacheAttnParams* ap, size_t* bytes) {
+  int dev = 0, max_lds = 0, cus = 0;
+  if (int rc = check_hip(hipGetDevice(&dev), "hipGetDevice")) return rc;
+  if (int rc = check_hip(hipDeviceGetAttribute(&max_lds, hipDeviceAttributeMaxSharedMemoryPerBlock,
+                                               dev),
+                         "hipDeviceGetAttribute"))
+    return rc;
+  if (int rc = device_cus(&cus)) return rc;
+  *bytes = asa::cache_attn_plan(*ap, size_t(max_lds), cus);
+  const long long blocks = (long long)ap->B * ap->c.heads * ((ap->R + 15) / 16) *
+                           (ap->nsplit > 1 ? ap->nsplit : 1);
+  if (blocks >= (1LL << 31)) return fail(ASA_ERR_INVALID_ARGUMENT, "problem too large");
   return ASA_OK;
 }
 
@@ -697,6 +835,82 @@ int asa_check_nonfinite(int32_t dtype, int32_t count, const void* const* tensors
   hipError_t e = asa::launch_nonfinite(np, dtype, s);
   asa::profile_end(s);
   if (int rc = check_hip(e, "nonfinite kernel launch")) return rc;
+  return ok();
+}
+
+int asa_cache_query_sizes(const asa_cache* c, size_t* codes, size_t* params) {
+  asa::CachePool pool;
+  if (int rc = validate_cache(c, false, &pool)) return rc;
+  if (!codes || !params) return fail(ASA_ERR_INVALID_ARGUMENT, "an argument is NULL");
+  const size_t rows = size_t(pool.pages) * pool.heads * pool.page;
+  *codes = rows * 16 * pool.G;
+  *params = rows * 4 * pool.G;
+  return ok();
+}
+
+int asa_cache_write(const asa_cache* c, const asa_cache_tokens* t, const int32_t* counts,
+                    const void* k, const void* v, void* stream) {
+  asa::CacheRowsParams rp{};
+  if (int rc = validate_tokens(c, t, &rp)) return rc;
+  if (!k || !v) return fail(ASA_ERR_INVALID_ARGUMENT, "a tensor argument is NULL");
+  if (int rc = cache_strides(t->k_strides, c->kv_heads, t->n, c->head_dim, "k", &rp.lk)) return rc;
+  if (int rc = cache_strides(t->v_strides, c->kv_heads, t->n, c->head_dim, "v", &rp.lv)) return rc;
+  rp.limit = counts;
+  rp.k = k;
+  rp.v = v;
+  rp.chunks = whole_chunks(k, rp.lk, c->head_dim, t->dtype) &&
+              whole_chunks(v, rp.lv, c->head_dim, t->dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  asa::profile_begin("cache_write", s);
+  hipError_t e = asa::launch_cache_write(rp, t->dtype, s);
+  asa::profile_end(s);
+  if (int rc = check_hip(e, "cache write kernel launch")) return rc;
+  return ok();
+}
+
+int asa_cache_read(const asa_cache* c, const asa_cache_tokens* t, const int32_t* lengths, void* k,
+                   void* v, void* stream) {
+  asa::CacheRowsParams rp{};
+  if (int rc = validate_tokens(c, t, &rp)) return rc;
+  if (!k || !v || !lengths) return fail(ASA_ERR_INVALID_ARGUMENT, "a tensor argument is NULL");
+  rp.limit = lengths;
+  rp.ok = k;
+  rp.ov = v;
+  const asa::Lay l = contiguous(c->kv_heads, t->n, c->head_dim);
+  rp.chunks = whole_chunks(k, l, c->head_dim, t->dtype) && whole_chunks(v, l, c->head_dim, t->dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  asa::profile_begin("cache_read", s);
+  hipError_t e = asa::launch_cache_read(rp, t->dtype, s);
+  asa::profile_end(s);
+  if (int rc = check_hip(e, "cache read kernel launch")) return rc;
+  return ok();
+}
+
+int asa_cache_attention_workspace(const asa_cache* c, const asa_cache_query* a, size_t* bytes) {
+  asa::CacheAttnParams ap{};
+  if (int rc = validate_query(c, a, false, &ap)) return rc;
+  if (!bytes) return fail(ASA_ERR_INVALID_ARGUMENT, "an argument is NULL");
+  if (int rc = plan_query(&ap, bytes)) return rc;
+  return ok();
+}
+
+int asa_cache_attention(const asa_cache* c, const asa_cache_query* a, const void* q, void* out,
+                        void* workspace, void* stream) {
+  asa::CacheAttnParams ap{};
+  if (int rc = validate_query(c, a, true, &ap)) return rc;
+  if (!q || !out) return fail(ASA_ERR_INVALID_ARGUMENT, "a tensor argument is NULL");
+  size_t bytes = 0;
+  if (int rc = plan_query(&ap, &bytes)) return rc;
+  if (bytes && !workspace) return fail(ASA_ERR_INVALID_ARGUMENT, "workspace is NULL");
+  if (int rc = check_aligned({workspace})) return rc;
+  ap.q = q;
+  ap.chunks = whole_chunks(q, ap.lq, c->head_dim, a->dtype);
+  ap.out = out;
+  ap.scores = static_cast<float*>(workspace);
+  ap.smax = ap.scores + size_t(ap.B) * ap.c.heads * ap.R * ap.span * ap.nsplit;
+  if (int rc = check_hip(asa::launch_cache_attn(ap, a->dtype, static_cast<hipStream_t>(stream)),
+                         "cache attention kernel launch"))
+    return rc;
   return ok();
 }
 

@@ -14,6 +14,9 @@ Drop-in for mvideet/Adaptive-Splash-Attention:
   the reference does (:669-676) and returns the reference kernel's
   gradient.
 * ``splash_attention`` -- functional form with autograd.
+* ``QuantizedKVCache`` and ``cache_attention`` -- serving: a paged key/value
+  cache held in 4 bits, written token by token, and the alpha-entmax
+  attention that reads it (no reference counterpart).
 
 All compute runs in hand-written HIP kernels in ``lib/libadasplash.so``;
 there is no CPU or PyTorch fallback.
@@ -26,14 +29,17 @@ import torch
 
 from . import ops
 from ._lib import ASAError
+from .cache import QuantizedKVCache, cache_attention
 from .function import SplashAttentionFunction, splash_attention
 from .module import AdaptiveSplashAttention
 
 __all__ = [
     "AdaptiveSplashAttention",
     "ASAError",
+    "QuantizedKVCache",
     "SplashAttentionFunction",
     "backward",
+    "cache_attention",
     "forward",
     "ops",
     "splash_attention",

@@ -45,6 +45,11 @@ EXPORTS = (
     "asa_backward",
     "asa_select_from_scores",
     "asa_check_nonfinite",
+    "asa_cache_query_sizes",
+    "asa_cache_write",
+    "asa_cache_read",
+    "asa_cache_attention_workspace",
+    "asa_cache_attention",
     "asa_set_pairing",
     "asa_profile_enable",
     "asa_profile_read",
@@ -93,6 +98,32 @@ class Sizes(ctypes.Structure):
     _fields_ = [(n, ctypes.c_size_t) for n in (
         "taus", "norms", "mask", "q_ptr", "q_list", "k_ptr", "k_list", "topk_idx", "topk_val",
         "sup_mask", "workspace")]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("pages", "kv_heads", "page_size", "head_dim")] + [
+        (n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_params", "v_params")]
+
+
+class CacheTokens(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "n", "dtype", "max_pages")] + [
+        ("page_table", ctypes.c_void_p),
+        ("start", ctypes.c_void_p),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+    ]
+
+
+class CacheQuery(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "heads", "nq", "dtype", "max_pages",
+                                              "max_length")] + [
+        ("alpha", ctypes.c_float),
+        ("sm_scale", ctypes.c_float),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("q_idx", ctypes.c_void_p),
+        ("q_strides", ctypes.c_int64 * 3),
+    ]
 
 
 class ASAError(RuntimeError):
@@ -151,6 +182,16 @@ def load() -> ctypes.CDLL:
                                                ctypes.POINTER(State), _V, _V]
         lib.asa_check_nonfinite.restype = ctypes.c_int
         lib.asa_check_nonfinite.argtypes = [_I, _I, _V, _V, _V, _V]
+        cache, tokens, query = (ctypes.POINTER(c) for c in (Cache, CacheTokens, CacheQuery))
+        size = ctypes.POINTER(ctypes.c_size_t)
+        for name, args in (("query_sizes", [cache, size, size]),
+                           ("write", [cache, tokens, _V, _V, _V, _V]),
+                           ("read", [cache, tokens, _V, _V, _V, _V]),
+                           ("attention_workspace", [cache, query, size]),
+                           ("attention", [cache, query, _V, _V, _V, _V])):
+            fn = getattr(lib, "asa_cache_" + name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = args
         lib.asa_set_pairing.restype = ctypes.c_int
         lib.asa_set_pairing.argtypes = [ctypes.c_int]
         lib.asa_profile_enable.restype = ctypes.c_int

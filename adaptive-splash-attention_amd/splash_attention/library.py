@@ -120,3 +120,80 @@ def attention(Q: Tensor, K: Tensor, V: Tensor, Q_idx: Optional[Tensor], K_idx: O
     out = forward_op(Q, K, V, Q_idx, K_idx, float(alpha), int(k_keep), float(sm_scale),
                      grad_mode, tau_mode, int(block_m), bwd_passes)[0]
     return ops.from_kernel_layout(out, Q.size(-1), Q.dtype)
+
+
+# ---------------------------------------------------------------------------
+# The 4-bit cache (cache.py).  A cache is passed as its four tensors, which the
+# write changes in place, and its head dimension.
+# ---------------------------------------------------------------------------
+
+def _cache(k_codes, k_params, v_codes, v_params, head_dim):
+    from .cache import QuantizedKVCache
+    return QuantizedKVCache.from_tensors(k_codes, k_params, v_codes, v_params, head_dim)
+
+
+@torch.library.custom_op(f"{_NS}::cache_write", device_types="cuda",
+                         mutates_args=("k_codes", "k_params", "v_codes", "v_params"))
+def cache_write_op(k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor,
+                   head_dim: int, K: Tensor, V: Tensor, page_table: Tensor, start: Tensor,
+                   counts: Optional[Tensor]) -> None:
+    """QuantizedKVCache.write."""
+    from . import cache
+    cache.write_tokens(_cache(k_codes, k_params, v_codes, v_params, head_dim), K, V, page_table,
+                       start, counts)
+
+
+@cache_write_op.register_fake
+def _cache_write_fake(k_codes, k_params, v_codes, v_params, head_dim, K, V, page_table, start,
+                      counts):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::cache_read", mutates_args=(), device_types="cuda")
+def cache_read_op(k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor,
+                  head_dim: int, page_table: Tensor, lengths: Tensor, n: int, dtype: torch.dtype,
+                  start: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """QuantizedKVCache.read."""
+    from . import cache
+    return cache.read_tokens(_cache(k_codes, k_params, v_codes, v_params, head_dim), page_table,
+                             lengths, n, dtype, start)
+
+
+@cache_read_op.register_fake
+def _cache_read_fake(k_codes, k_params, v_codes, v_params, head_dim, page_table, lengths, n, dtype,
+                     start):
+    shape = (page_table.shape[0], k_codes.shape[1], n, head_dim)
+    return (torch.empty(shape, dtype=dtype, device=k_codes.device),
+            torch.empty(shape, dtype=dtype, device=k_codes.device))
+
+
+@torch.library.custom_op(f"{_NS}::cache_attention", mutates_args=(), device_types="cuda")
+def cache_attention_op(k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor,
+                       head_dim: int, Q: Tensor, page_table: Tensor, lengths: Tensor,
+                       Q_idx: Optional[Tensor], alpha: float, sm_scale: float,
+                       max_length: Optional[int]) -> Tensor:
+    """cache_attention."""
+    from . import cache
+    return cache.attend(_cache(k_codes, k_params, v_codes, v_params, head_dim), Q, page_table,
+                        lengths, Q_idx, alpha, sm_scale, max_length)
+
+
+@cache_attention_op.register_fake
+def _cache_attention_fake(k_codes, k_params, v_codes, v_params, head_dim, Q, page_table, lengths,
+                          Q_idx, alpha, sm_scale, max_length):
+    return torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
+
+
+def cache_write(cache, K, V, page_table, start, counts) -> None:
+    cache_write_op(*cache.tensors(), cache.head_dim, K, V, page_table, start, counts)
+
+
+def cache_read(cache, page_table, lengths, n, dtype, start):
+    if n is None:
+        n = page_table.shape[1] * cache.page_size
+    return cache_read_op(*cache.tensors(), cache.head_dim, page_table, lengths, int(n), dtype, start)
+
+
+def cache_attention(cache, Q, page_table, lengths, Q_idx, alpha, sm_scale, max_length) -> Tensor:
+    return cache_attention_op(*cache.tensors(), cache.head_dim, Q, page_table, lengths, Q_idx,
+                              alpha, sm_scale, None if max_length is None else int(max_length))

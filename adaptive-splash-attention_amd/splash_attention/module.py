@@ -5,6 +5,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from .cache import QuantizedKVCache, cache_attention
 from .function import splash_attention
 
 
@@ -81,3 +82,18 @@ class AdaptiveSplashAttention(nn.Module):
             raise ValueError(f"Q head dim {Q.size(-1)} != head_dim {self.head_dim}")
         return splash_attention(Q, K, V, Q_idx, K_idx, self.alpha, self.k_keep, self.sm_scale,
                                 self.grad_mode, self.tau_mode, self.block_m, self.bwd_passes)
+
+    def decode(self, Q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.Tensor,
+               lengths: torch.Tensor, Q_idx: torch.Tensor | None = None,
+               max_length: int | None = None) -> torch.Tensor:
+        """The module's attention of a few query tokens per sequence over a
+        4-bit cache (``cache_attention`` with its alpha and sm_scale; no
+        reference counterpart).  Needs ``tau_mode="exact"``: the top-k
+        threshold of the reference mode depends on which queries share a
+        block, which single tokens do not have."""
+        if self.tau_mode != "exact":
+            raise ValueError("decode needs tau_mode 'exact'")
+        if Q.size(-1) != self.head_dim:
+            raise ValueError(f"Q head dim {Q.size(-1)} != head_dim {self.head_dim}")
+        return cache_attention(Q, cache, page_table, lengths, Q_idx, self.alpha, self.sm_scale,
+                               max_length)

@@ -264,6 +264,98 @@ int asa_select_from_scores(const asa_problem *p, const float *scores, const int3
 int asa_check_nonfinite(int32_t dtype, int32_t count, const void* const* tensors,
                         const int64_t* elements, uint32_t* flags, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Serving: a paged key/value cache held in 4 bits (no reference counterpart;
+ * the reference has no cache).  Tokens are quantised as they are written,
+ * asa_cache_attention reads the codes in place, asa_cache_read gives the
+ * values they stand for.
+ *
+ * A row (one token's key or value of one head) is head_dim channels in
+ * G = ceil(head_dim / 32) groups of 32.  A group has a scale s and an offset
+ * m, both bf16, and per channel a code c of 4 bits that stands for m + c s:
+ *   m = the largest bf16 at most min(x)
+ *   s = the smallest bf16 >= 2^-126 with 15 s >= max(x) - m (0 if max(x) = m)
+ *   c = the number of borders m + (k + 1/2) s, k = 0..14, below x
+ * so every value is within s / 2 of the one written.  A NaN is written as 0,
+ * a value past +-2^126 as that bound.
+ *   codes   uint8  [pages, kv_heads, page_size, 16 G]: the dword of channels
+ *                  32 g + 8 o .. + 7 (nibble j: channel j of them) is dword
+ *                  4 g + o of a value row and dword G o + g of a key row;
+ *                  codes of channels past head_dim are 0
+ *   params  uint16 [pages, kv_heads, page_size, G, 2]: bf16 bits of s, m
+ * Every pointer is 16-byte aligned.  Position t of sequence b is row
+ * t % page_size of page page_table[b * max_pages + t / page_size].  A
+ * position past max_pages, or whose entry is not a page of the pool, has no
+ * row: it is not written, reads as zeros, and no query sees it.           */
+typedef struct asa_cache {
+  int32_t pages;     /* >= 1                                               */
+  int32_t kv_heads;
+  int32_t page_size; /* tokens of a page: 16, 32, 64, 128 or 256           */
+  int32_t head_dim;  /* 1..128                                             */
+  void *k_codes;
+  void *v_codes;
+  void *k_params;
+  void *v_params;
+} asa_cache;
+
+/* Bytes of each codes and each params tensor of the cache (the pointers are
+ * not looked at).  Host-only.                                              */
+int asa_cache_query_sizes(const asa_cache *c, size_t *codes, size_t *params);
+
+/* The tokens of a write or read: k and v [batch, kv_heads, n, head_dim].    */
+typedef struct asa_cache_tokens {
+  int32_t batch;
+  int32_t n;
+  int32_t dtype;             /* asa_dtype of k and v                       */
+  int32_t max_pages;         /* columns of page_table                      */
+  const int32_t *page_table; /* [batch, max_pages]                         */
+  const int32_t *start;      /* [batch] position of token 0 (NULL: 0)      */
+  int64_t k_strides[3];      /* write only: element strides {batch, head,  */
+  int64_t v_strides[3];      /* token}, >= 0; {0, 0, 0}: contiguous        */
+} asa_cache_tokens;
+
+/* Writes token i < counts[b] (NULL: n) of sequence b at position start[b] +
+ * i.  Rows of other positions are left as they are.  Two tokens of one call
+ * must not go to one row (sequences that share a page write to it in
+ * different calls): which of the two rows' bytes stay is not defined.      */
+int asa_cache_write(const asa_cache *c, const asa_cache_tokens *t, const int32_t *counts,
+                    const void *k, const void *v, void *stream);
+
+/* k and v (contiguous): the values at positions start[b] + i, i < n, rounded
+ * once to dtype; zeros at positions past lengths[b] or below 0.            */
+int asa_cache_read(const asa_cache *c, const asa_cache_tokens *t, const int32_t *lengths, void *k,
+                   void *v, void *stream);
+
+/* alpha-entmax attention (the exact threshold, as ASA_TAU_EXACT) of nq query
+ * tokens per sequence over its cached keys: q and out [batch, heads, nq,
+ * head_dim], heads a multiple of kv_heads (query head j reads key head j /
+ * (heads / kv_heads)).  Query token i at position q_idx[b, i] (NULL:
+ * lengths[b] - nq + i) sees the keys at positions <= its own and below
+ * lengths[b].  A row that sees no key gives zeros.  Scores are clamped to
+ * [-10, 10] as in asa_forward; a query row that holds a value that is not
+ * finite scores -10 throughout.                                            */
+typedef struct asa_cache_query {
+  int32_t batch;
+  int32_t heads;
+  int32_t nq;                /* 1..64                                      */
+  int32_t dtype;             /* asa_dtype of q and out                     */
+  int32_t max_pages;
+  int32_t max_length;        /* no lengths[b] counts for more than this
+                              * (0: max_pages * page_size); work and
+                              * workspace are sized by it                  */
+  float alpha;               /* clamped to [1.05, 3]                       */
+  float sm_scale;
+  const int32_t *page_table; /* [batch, max_pages]                         */
+  const int32_t *lengths;    /* [batch] cached tokens                      */
+  const int32_t *q_idx;      /* [batch, nq] or NULL                        */
+  int64_t q_strides[3];      /* as asa_cache_tokens.k_strides              */
+} asa_cache_query;
+
+/* Workspace bytes of the call (0: none needed).                            */
+int asa_cache_attention_workspace(const asa_cache *c, const asa_cache_query *a, size_t *bytes);
+int asa_cache_attention(const asa_cache *c, const asa_cache_query *a, const void *q, void *out,
+                        void *workspace, void *stream);
+
 /* Which forward kernel runs for 16-bit inputs (no reference counterpart;
  * for tuning and tests): ASA_PAIRING_AUTO (default) runs two query blocks
  * per workgroup when those workgroups fill at least one wave of the GPU
