@@ -84,13 +84,12 @@ struct CacheAttnParams {
   int plan;               // CachePlan
   int span, nsplit;       // split plan: keys per score block, score blocks per row tile
   float* scores;          // split plan: [B * c.heads * R, span * nsplit]
-  float* smax;            // split plan: [B * c.heads * R, nsplit]
 };
 // How attention runs: one block per 16 rows that holds their scores in LDS,
 // or the keys split over score blocks, then one block per row.
 enum CachePlan : int { kCacheOneBlock = 0, kCacheSplit = 1 };
 // Fills plan, span and nsplit; returns the workspace bytes.
-size_t cache_attn_plan(CacheAttnParams& p, size_t max_lds, int cus);
+size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus);
 hipError_t launch_cache_attn(const CacheAttnParams& p, int dtype, hipStream_t s);
 
 }  // namespace asa

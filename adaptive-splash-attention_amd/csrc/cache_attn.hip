@@ -20,11 +20,13 @@
 // type.
 //
 // tau lies in [max z - 1, max z], so only keys with z > max z - 1 can have a
-// weight: they are listed (index, z) in LDS, Newton steps over the list find
-// tau, and only the value rows of the support are read, by their entry in
-// the list.  alpha-entmax gives most keys of a long row no weight, so the
-// values' bytes are a small part of the keys'.
+// weight.  A row's z are held in registers, the candidates are listed (index,
+// z) in LDS, Newton steps over the list find tau, and only the value rows of
+// the support are read, by their entry in the list.  alpha-entmax gives most
+// keys of a long row no weight, so the values' bytes are a small part of the
+// keys'.  Lists have a fixed order, so results do not depend on timing.
 #include <climits>
+#include <type_traits>
 
 #include "asa_cache.hpp"
 #include "asa_device.hpp"
@@ -32,9 +34,8 @@
 namespace asa {
 namespace {
 
-constexpr float kHidden = -3e38f;  // z of a key that a row does not see
-constexpr int kRows = 16;          // query rows of an MFMA tile
-constexpr int kSub = 16;           // keys of an MFMA tile
+constexpr float kHidden = -3e38f;  // score of a key that a row does not see
+constexpr int kTile = 16;          // rows and keys of an MFMA tile
 
 // ---------------------------------------------------------------------------
 // Scores
@@ -47,22 +48,53 @@ __device__ __forceinline__ int visible_keys(const CacheAttnParams& p, int b, int
   return at < 0 ? 0 : at >= len ? len : at + 1;
 }
 
-// One wave's query operand: rows r0 .. r0 + 15 of a key head's R rows (row
-// r: query head h * rep + r / NQ, token r % NQ) as NT bf16 terms per group,
-// the accumulators' starts, and the offsets' operand.
-template <typename T, int NT, int NG>
+// The 16-bit format of the codes operand: fp16 for fp16 queries, else bf16.
+template <typename T> using CodeType = typename std::conditional<std::is_same<T, h16>::value, h16, u16>::type;
+template <typename T> using CodeVec = typename Half<CodeType<T>>::v8;
+
+// 8 codes as 16 + c: channels 0 4 1 5 2 6 3 7, since nibbles j and j + 4 are
+// 16 bits apart.  The query operand has the same order.
+__device__ __forceinline__ int operand_slot(int j) { return j < 4 ? 2 * j : 2 * j - 7; }
+template <typename T> __device__ __forceinline__ CodeVec<T> codes_operand(uint32_t w) {
+  uint32_t u[4];
+  if constexpr (std::is_same<T, h16>::value) {  // 16.0 = 0x4c00, one = 1 << 6
+    const uint32_t mask = 0x03c003c0u, one = 0x4c004c00u;
+    u[0] = ((w << 6) & mask) | one;
+    u[1] = ((w << 2) & mask) | one;
+    u[2] = ((w >> 2) & mask) | one;
+    u[3] = ((w >> 6) & mask) | one;
+  } else {  // 16.0 = 0x4180, one = 1 << 3
+    const uint32_t mask = 0x00780078u, one = 0x41804180u;
+    u[0] = ((w << 3) & mask) | one;
+    u[1] = ((w >> 1) & mask) | one;
+    u[2] = ((w >> 5) & mask) | one;
+    u[3] = ((w >> 9) & mask) | one;
+  }
+  CodeVec<T> r;
+  __builtin_memcpy(&r, u, 16);
+  return r;
+}
+
+// One wave's query operand: rows r0 .. of a key head's R rows (row r: query
+// head h * rep + r / NQ, token r % NQ), kR of them, for each of the P key
+// tiles that share a result, and the accumulators' starts.  Queries of a
+// negative scale are negated, so that larger products are larger scores.
+template <typename T, int P, int NG>
 struct QueryFrag {
-  bf16x8 a[NG][NT];
-  f32x4 bias[NG];
-  bf16x8 am;
-  int vis[4];  // visible keys of rows 4 (lane / 16) + r
+  static constexpr int kR = kTile / P;
+  static constexpr int NT = std::is_same<T, float>::value ? 3 : 1;
+  CodeVec<T> a[P][NG][NT];
+  f32x4 bias[NG];  // -16 sum q_g of rows (4 (lane / 16) + k) % kR
+  int vis[4];      // visible keys of those rows
+  int most, least; // over the real rows of the tile
 
   __device__ __forceinline__ void load(const CacheAttnParams& p, int b, int h, int r0, int lane) {
-    const int o = lane >> 4, r = r0 + (lane & 15);
+    using S = typename Half<CodeType<T>>::scalar;
+    const int o = lane >> 4, ar = lane & 15, r = r0 + ar % kR;
     const bool ok = r < p.R;
     const int rr = ok ? r : 0, head = h * p.rep + rr / p.NQ, i = rr % p.NQ;
     const T* q = static_cast<const T*>(p.q) + size_t(b) * p.lq.sb + size_t(head) * p.lq.sh + size_t(i) * p.lq.sn;
-    float sum[NG];
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const int ch = 32 * g + 8 * o, nv = ok ? p.c.hd - ch : 0;
@@ -79,94 +111,94 @@ struct QueryFrag {
       } else {
         for (int j = 0; j < 8; ++j) x[j] = j < nv ? Elem<T>::load(q + ch + j) : 0.0f;
       }
-      float t = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-      sum[g] = sum_groups(t);
+      for (int j = 0; j < 8; ++j) x[j] *= sign;
+      const float sum = sum_groups(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
+      for (int k = 0; k < 4; ++k) bias[g][k] = -16.0f * __shfl(sum, 4 * o + k, 64);
 #pragma unroll
-      for (int k = 0; k < NT; ++k)
+      for (int t = 0; t < NT; ++t)
         for (int j = 0; j < 8; ++j) {
-          const __bf16 y = static_cast<__bf16>(x[j]);
-          a[g][k][j < 4 ? 2 * j : 2 * j - 7] = y;  // codes_operand's order
+          const S y = static_cast<S>(x[j]);
           x[j] -= static_cast<float>(y);
+          for (int u = 0; u < P; ++u) a[u][g][t][operand_slot(j)] = ar / kR == u ? y : static_cast<S>(0.0f);
         }
-      for (int k = 0; k < 4; ++k) bias[g][k] = -16.0f * __shfl(sum[g], 4 * o + k, 64);
     }
-    // sum q_g in three bf16 terms (24 bits) against m_g: slots of lane group
-    // 0 hold the first two terms of four groups, those of group 1 the third
-    for (int j = 0; j < 8; ++j) am[j] = static_cast<__bf16>(0.0f);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const __bf16 s0 = static_cast<__bf16>(sum[g]);
-      const float r1 = sum[g] - static_cast<float>(s0);
-      const __bf16 s1 = static_cast<__bf16>(r1);
-      const __bf16 s2 = static_cast<__bf16>(r1 - static_cast<float>(s1));
-      if (o == 0) am[g] = s0, am[4 + g] = s1;
-      if (o == 1) am[g] = s2;
-    }
+    int hi = 0, lo = INT_MAX;
     for (int k = 0; k < 4; ++k) {
-      const int row = r0 + 4 * o + k;
+      const int row = r0 + (4 * o + k) % kR;
       vis[k] = row < p.R ? visible_keys(p, b, row % p.NQ) : 0;
+      hi = max(hi, vis[k]);
+      lo = row < p.R ? min(lo, vis[k]) : lo;
     }
+    most = wave_reduce_minmax<true>(hi);
+    least = wave_reduce_minmax<false>(lo);
   }
 };
 
-// The codes (key order: lane group o has octet o of every group) and params
-// of the lane's key.
-template <int NG>
-struct KeyRow {
-  uint32_t w[NG], pr[NG];
-  __device__ __forceinline__ void load(const CachePool& c, int64_t row, int o) {
-    const uint32_t* cw = reinterpret_cast<const uint32_t*>(c.k_codes) + row * (4 * NG) + NG * o;
-    const uint32_t* cp = c.k_params + row * NG;
-    __builtin_memcpy(w, __builtin_assume_aligned(cw, NG == 4 ? 16 : NG == 2 ? 8 : 4), 4 * NG);
-    __builtin_memcpy(pr, __builtin_assume_aligned(cp, NG == 4 ? 16 : NG == 2 ? 8 : 4), 4 * NG);
+// P tiles of 16 keys: the codes (key order: lane group o has octet o of every
+// channel group) of key lane % 16 of each tile, and the params of the lane's
+// own key of the result.
+template <int P, int NG>
+struct KeyPack {
+  uint32_t w[P][NG], pr[NG];
+  bool seen;  // the lane's own key has a page
+
+  template <int N> static __device__ __forceinline__ void words(uint32_t* d, const uint32_t* s) {
+    __builtin_memcpy(d, __builtin_assume_aligned(s, N == 4 ? 16 : N == 2 ? 8 : 4), 4 * N);
+  }
+  // keys base .. base + 16 P - 1 of [.., key1); pages: of the keys from key0
+  __device__ __forceinline__ void load(const CachePool& c, int h, const int* pages, int key0, int base, int key1,
+                                       int lane) {
+    const int o = lane >> 4, col = lane & 15;
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+      const int key = base + kTile * u;
+      const int pg = key < key1 ? __builtin_amdgcn_readfirstlane(pages[(key - key0) >> c.page_shift]) : -1;
+      if (pg >= 0) {
+        const int64_t row = (int64_t(pg) * c.heads + h) * c.page + (key & (c.page - 1)) + col;
+        words<NG>(w[u], reinterpret_cast<const uint32_t*>(c.k_codes) + row * (4 * NG) + NG * o);
+      } else {
+        for (int g = 0; g < NG; ++g) w[u][g] = 0u;
+      }
+    }
+    const int key = base + kTile * (o * P / 4);
+    const int pg = key < key1 ? pages[(key - key0) >> c.page_shift] : -1;
+    seen = pg >= 0;
+    for (int g = 0; g < NG; ++g) pr[g] = 0u;
+    if (seen) words<NG>(pr, c.k_params + ((int64_t(pg) * c.heads + h) * c.page + (key & (c.page - 1)) + col) * NG);
   }
 };
 
-// 8 codes as bf16 16 + c: channels 0 4 1 5 2 6 3 7, since nibbles j and j + 4
-// are 16 bits apart.  The query operand has the same order.
-__device__ __forceinline__ bf16x8 codes_operand(uint32_t w) {
-  const uint32_t mask = 0x00780078u, one = 0x41804180u;
-  uint32_t u[4];
-  u[0] = ((w << 3) & mask) | one;
-  u[1] = ((w >> 1) & mask) | one;
-  u[2] = ((w >> 5) & mask) | one;
-  u[3] = ((w >> 9) & mask) | one;
-  bf16x8 r;
-  __builtin_memcpy(&r, u, 16);
-  return r;
-}
-
-// q.k of 16 rows x 16 keys: element r of a lane is row 4 (lane / 16) + r,
-// key lane % 16.
-template <typename T, int NT, int NG>
-__device__ __forceinline__ f32x4 dots(const QueryFrag<T, NT, NG>& q, const KeyRow<NG>& k) {
-  uint32_t mm[4] = {};
+// q.k: element k of a lane is row (4 (lane / 16) + k) % kR, key
+// 16 (lane / 16 * P / 4) + lane % 16 of the pack.
+template <typename T, int P, int NG>
+__device__ __forceinline__ f32x4 dots(const QueryFrag<T, P, NG>& q, const KeyPack<P, NG>& k) {
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    const uint32_t m = k.pr[g] >> 16;
-    mm[g >> 1] |= (g & 1) ? (k.pr[g] & 0xffff0000u) : m;
-  }
-  mm[2] = mm[0], mm[3] = mm[1];
-  bf16x8 bm;
-  __builtin_memcpy(&bm, mm, 16);
-  f32x4 s = mfma(q.am, bm, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const bf16x8 u = codes_operand(k.w[g]);
     f32x4 acc = q.bias[g];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) acc = mfma(q.a[g][t], u, acc);
+    for (int u = 0; u < P; ++u) {
+      const CodeVec<T> c = codes_operand<T>(k.w[u][g]);
+#pragma unroll
+      for (int t = 0; t < QueryFrag<T, P, NG>::NT; ++t) acc = mfma(q.a[u][g][t], c, acc);
+    }
     const float sc = __uint_as_float(k.pr[g] << 16);
-    for (int r = 0; r < 4; ++r) s[r] = fmaf(sc, acc[r], s[r]);
+    const float off = __uint_as_float(k.pr[g] & 0xffff0000u) * -0.0625f;  // m sum q_g = -m / 16 bias
+    for (int r = 0; r < 4; ++r) s[r] = fmaf(off, q.bias[g][r], fmaf(sc, acc[r], s[r]));
   }
   return s;
 }
 
-// z = (alpha - 1) clamp(scale dot); a dot that is not a number counts as the
-// lower bound, as in the score clamp of the dense path.
-__device__ __forceinline__ float z_of(float dot, float c, float zb) {
-  return __builtin_amdgcn_fmed3f(dot * c, -zb, zb);
-}
+// z = (alpha - 1) clamp(|scale| dot), hidden keys apart; a dot that is not a
+// number counts as the lower bound, as in the score clamp of the dense path.
+struct ZOf {
+  float c, zb;
+  __device__ __forceinline__ explicit ZOf(const CacheAttnParams& p)
+      : c((p.alpha - 1.0f) * fabsf(p.scale)), zb(10.0f * (p.alpha - 1.0f)) {}
+  __device__ __forceinline__ float operator()(float dot) const {
+    return dot == kHidden ? kHidden : __builtin_amdgcn_fmed3f(dot * c, -zb, zb);
+  }
+};
 
 // Pages of the keys [key0, key0 + n) into LDS (-1: none that the pool has).
 __device__ __forceinline__ void stage_pages(const CacheAttnParams& p, int b, int key0, int n,
@@ -179,34 +211,36 @@ __device__ __forceinline__ void stage_pages(const CacheAttnParams& p, int b, int
   }
 }
 
-// z of the keys [key0, key1) x 16 rows by the block's waves, 16 U keys per
-// wave and step, handed to put(r, key, z) (row 4 (lane / 16) + r of the
-// tile).  key0 is a multiple of the page size; pages: stage_pages of it.
-template <int U, int NW, typename T, int NT, int NG, typename Put>
-__device__ __forceinline__ void score_keys(const CacheAttnParams& p, const QueryFrag<T, NT, NG>& q, int h,
+// Dots of the keys [key0, key1) by the block's NW waves, V packs per wave in
+// flight, handed to put(key, dots) (dots as from `dots`; hidden where a row
+// does not see the key).  key0 is a multiple of the page size.
+template <int V, int NW, typename T, int P, int NG, typename Put>
+__device__ __forceinline__ void score_keys(const CacheAttnParams& p, const QueryFrag<T, P, NG>& q, int h,
                                            int key0, int key1, const int* pages, int w, int lane,
                                            Put put) {
-  const float zc = (p.alpha - 1.0f) * p.scale, zb = 10.0f * (p.alpha - 1.0f);
-  const int o = lane >> 4, kl = lane & 15;
-  for (int base = key0 + w * (kSub * U); base < key1; base += NW * (kSub * U)) {
-    KeyRow<NG> kr[U];
-    bool on[U];
+  constexpr int kKeys = kTile * P, kStep = NW * V * kKeys;
+  const int own = kTile * ((lane >> 4) * P / 4) + (lane & 15);
+  KeyPack<P, NG> next[V];
+  int base = key0 + w * (V * kKeys);
+  if (base < key1)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int key = base + kSub * u;
-      const int pg = key < key1 ? __builtin_amdgcn_readfirstlane(pages[(key - key0) >> p.c.page_shift]) : -1;
-      on[u] = pg >= 0;
-      if (on[u])
-        kr[u].load(p.c, (int64_t(pg) * p.c.heads + h) * p.c.page + (key & (p.c.page - 1)) + kl, o);
-    }
+    for (int v = 0; v < V; ++v) next[v].load(p.c, h, pages, key0, base + v * kKeys, key1, lane);
+  for (; base < key1; base += kStep) {
+    KeyPack<P, NG> k[V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int key = base + kSub * u + kl;
-      if (on[u]) {
-        const f32x4 d = dots<T, NT, NG>(q, kr[u]);
-        for (int r = 0; r < 4; ++r) put(r, key, key < q.vis[r] ? z_of(d[r], zc, zb) : kHidden);
-      } else if (base + kSub * u < key1) {
-        for (int r = 0; r < 4; ++r) put(r, key, kHidden);
+    for (int v = 0; v < V; ++v) k[v] = next[v];
+    if (base + kStep < key1)
+#pragma unroll
+      for (int v = 0; v < V; ++v) next[v].load(p.c, h, pages, key0, base + kStep + v * kKeys, key1, lane);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int first = base + v * kKeys, key = first + own;
+      if (first < key1) {
+        f32x4 d = dots<T, P, NG>(q, k[v]);
+        if (first + kKeys > q.least)
+          for (int r = 0; r < 4; ++r) d[r] = key < q.vis[r] ? d[r] : kHidden;
+        for (int r = 0; r < 4; ++r) d[r] = k[v].seen ? d[r] : kHidden;
+        put(key, d);
       }
     }
   }
@@ -216,21 +250,30 @@ __device__ __forceinline__ void score_keys(const CacheAttnParams& p, const Query
 // Threshold and values of one row by a team of waves
 // ---------------------------------------------------------------------------
 
+template <typename F> __device__ __forceinline__ float wave_reduce(float v, F op) {
+  v = op(v, __uint_as_float(lane_xor<1>(__float_as_uint(v))));
+  v = op(v, __uint_as_float(lane_xor<2>(__float_as_uint(v))));
+  v = op(v, __uint_as_float(lane_xor<7>(__float_as_uint(v))));
+  v = op(v, __uint_as_float(lane_xor<15>(__float_as_uint(v))));
+  return __uint_as_float(group_reduce_bits(__float_as_uint(v), [op](uint32_t x, uint32_t y) {
+    return __float_as_uint(op(__uint_as_float(x), __uint_as_float(y)));
+  }));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-  v += __uint_as_float(lane_xor<1>(__float_as_uint(v)));
-  v += __uint_as_float(lane_xor<2>(__float_as_uint(v)));
-  v += __uint_as_float(lane_xor<7>(__float_as_uint(v)));
-  v += __uint_as_float(lane_xor<15>(__float_as_uint(v)));
-  return sum_groups(v);
+  return wave_reduce(v, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ float wave_max(float v) {
-  v = fmaxf(v, __uint_as_float(lane_xor<1>(__float_as_uint(v))));
-  v = fmaxf(v, __uint_as_float(lane_xor<2>(__float_as_uint(v))));
-  v = fmaxf(v, __uint_as_float(lane_xor<7>(__float_as_uint(v))));
-  v = fmaxf(v, __uint_as_float(lane_xor<15>(__float_as_uint(v))));
-  return __uint_as_float(group_reduce_bits(__float_as_uint(v), [](uint32_t x, uint32_t y) {
-    return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
-  }));
+  return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+// Sum over the lanes up to and with the calling one.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
 }
 
 // v^e and v^(e-1), v >= 0, both 0 at v = 0.
@@ -270,27 +313,26 @@ __device__ __forceinline__ bool next_tau(float alpha, float F, float F1, float& 
 }
 constexpr int kMaxSteps = 64;
 
-// LDS of the row teams: a candidate list and partial sums for each wave.
+// LDS of the row teams: each wave's share of its team's candidate list, and
+// partial results.
+constexpr int kAccStride = 132;
 struct TeamLds {
-  float* lz;   // [NW][cap] z, later p
-  int* li;     // [NW][cap] key
+  float* lz;   // [NW * cap] z, later p
+  int* li;     // [NW * cap] key
   float* red;  // [NW][4]
   int* cnt;    // [NW]
   float* acc;  // [NW][kAccStride]
-  int cap;
 };
-constexpr int kAccStride = 132;
-template <int NW> __host__ __device__ inline size_t team_lds_bytes(int cap) {
-  return size_t(NW) * (size_t(cap) * 8 + 16 + 4 + kAccStride * 4);
+template <int NW, int CAP> constexpr size_t team_lds_bytes() {
+  return size_t(NW) * (size_t(CAP) * 8 + 16 + 4 + kAccStride * 4);
 }
-template <int NW> __device__ __forceinline__ TeamLds team_lds(void* base, int cap) {
+template <int NW, int CAP> __device__ __forceinline__ TeamLds team_lds(void* base) {
   TeamLds l;
   l.lz = static_cast<float*>(base);
-  l.li = reinterpret_cast<int*>(l.lz + NW * cap);
-  l.red = reinterpret_cast<float*>(l.li + NW * cap);
+  l.li = reinterpret_cast<int*>(l.lz + NW * CAP);
+  l.red = reinterpret_cast<float*>(l.li + NW * CAP);
   l.cnt = reinterpret_cast<int*>(l.red + NW * 4);
   l.acc = reinterpret_cast<float*>(l.cnt + NW);
-  l.cap = cap;
   return l;
 }
 
@@ -334,7 +376,7 @@ struct ValueSum {
       }
     }
   }
-  // the wave's sums of channels 8 c + j, in the lanes of slot 0
+  // the wave's sums of channels 8 c + j, in every lane with that c
   __device__ __forceinline__ void reduce() {
     for (int j = 0; j < 8; ++j) {
       acc[j] += off;
@@ -345,18 +387,49 @@ struct ValueSum {
   }
 };
 
-// tau and the output of row `row` (of the key head's R) from its z at zp[0 ..
-// vis), by `size` waves of the block, of which this is number `member`; its
-// waves are w0 .. w0 + size - 1.  Every wave of the block calls it together
-// (teams meet at the block's barriers); vis = 0 for a team without a row.
-// zpart: the wave's part of the row's maximum.
-template <typename T, int NG, int NW>
+// tau and the output of row `row` (of the key head's R) from its dots at
+// sp[0 .. vis) (16-byte aligned), by `size` waves of the block from wave w0
+// on.  Every wave of the block calls it together (teams meet at the block's
+// barriers); row = -1, vis = 0 for a team without a row.  A lane holds 32 z
+// at a time: rows of at most 2048 * size keys stay in registers, longer ones
+// are read again at each step.
+constexpr int kQuads = 8;  // 16-byte loads of a lane
+template <typename T, int NG, int NW, int CAP>
 __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int h, int row, int vis,
-                                           const float* zp, float zpart, const TeamLds& L, int w, int w0,
-                                           int size, int lane) {
+                                           const float* sp, const TeamLds& L, int w, int w0, int size,
+                                           int lane) {
   const int member = w - w0;
   const float e = 1.0f / (p.alpha - 1.0f);
   const int pc = pow_class_of(e);
+  const ZOf zof(p);
+  const int seg = size * kWave * 4 * kQuads;
+  const bool once = vis <= seg;
+  float z[4 * kQuads];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+      const int at = s0 + ((q * size + member) * kWave + lane) * 4;
+      float4 f = float4{kHidden, kHidden, kHidden, kHidden};
+      if (at < vis) f = *reinterpret_cast<const float4*>(sp + at);
+      z[4 * q] = at < vis ? zof(f.x) : kHidden;
+      z[4 * q + 1] = at + 1 < vis ? zof(f.y) : kHidden;
+      z[4 * q + 2] = at + 2 < vis ? zof(f.z) : kHidden;
+      z[4 * q + 3] = at + 3 < vis ? zof(f.w) : kHidden;
+    }
+  };
+  // body(key of z[0], z) over the row's parts; z[4 q + j]: 256 size q + j further
+  auto sweep = [&](auto body) {
+    for (int s0 = 0; s0 < vis; s0 += seg) {
+      if (!once) fetch(s0);
+      body(s0 + (member * kWave + lane) * 4);
+    }
+  };
+  if (once) fetch(0);
+  float zpart = kHidden;
+  sweep([&](int) {
+#pragma unroll
+    for (int k = 0; k < 4 * kQuads; ++k) zpart = fmaxf(zpart, z[k]);
+  });
   const float wm = wave_max(zpart);
   if (lane == 0) L.red[4 * w] = wm;
   __syncthreads();
@@ -365,41 +438,58 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
   const bool empty = !(zmax > 0.5f * kHidden);
   float tau = zmax - 1.0f, lo = tau, hi = zmax;
 
-  // ---- the keys with z > lo, listed per wave; lo moves up while they do not fit ----
-  float* lz = L.lz + w * L.cap;
-  int* li = L.li + w * L.cap;
+  // ---- the keys with z > lo, listed; lo moves up while they do not fit ----
+  float* lz = L.lz + w0 * CAP;
+  int* li = L.li + w0 * CAP;
   bool listed = false, dense = empty;
-  int mine = 0;
+  int n = 0;
   for (int it = 0;; ++it) {
+    int mine = 0, upto = 0;
     if (!listed && !dense) {
-      mine = 0;
-      for (int j0 = member * kWave; j0 < vis; j0 += size * kWave) {
-        const float z = j0 + lane < vis ? zp[j0 + lane] : kHidden;
-        const uint64_t m = __ballot(z > lo);
-        const int at = mine + lane_rank(m);
-        if (z > lo && at < L.cap) {
-          lz[at] = z;
-          li[at] = j0 + lane;
-        }
-        mine += __builtin_popcountll(m);
-      }
-      if (lane == 0) L.cnt[w] = mine;
+      sweep([&](int) {
+#pragma unroll
+        for (int k = 0; k < 4 * kQuads; ++k) mine += z[k] > lo ? 1 : 0;
+      });
+      upto = wave_scan(mine);
+      if (lane == kWave - 1) L.cnt[w] = upto;
     }
     __syncthreads();
     if (!listed && !dense) {
-      listed = true;
-      for (int i = 0; i < size; ++i) listed = listed && L.cnt[w0 + i] <= L.cap;
+      n = 0;
+      int before = 0;
+      for (int i = 0; i < size; ++i) {
+        if (i == member) before = n;
+        n += L.cnt[w0 + i];
+      }
+      listed = n <= size * CAP;
+      if (listed) {
+        int at = before + upto - mine;
+        sweep([&](int key) {
+          if (mine)
+#pragma unroll
+            for (int k = 0; k < 4 * kQuads; ++k)
+              if (z[k] > lo) {
+                lz[at] = z[k];
+                li[at] = key + (k >> 2) * (size * kWave * 4) + (k & 3);
+                ++at;
+              }
+        });
+      }
     }
     if (!__syncthreads_or(!listed && !dense)) break;
     // some team's candidates did not fit: one step of its tau over the whole row
     float F = 0.0f, F1 = 0.0f;
     if (!listed && !dense) {
-      for (int j0 = member * kWave; j0 < vis; j0 += size * kWave) {
-        const float z = j0 + lane < vis ? zp[j0 + lane] : kHidden;
-        float pa, pa1;
-        powers(pc, fmaxf(z - tau, 0.0f), e, pa, pa1);
-        F += pa;
-        F1 += pa1;
+#pragma unroll 2
+      for (int at = (member * kWave + lane) * 4; at < vis; at += size * kWave * 4) {
+        const float4 f = *reinterpret_cast<const float4*>(sp + at);
+        const float d[4] = {f.x, f.y, f.z, f.w};
+        for (int j = 0; j < 4; ++j) {
+          float pa, pa1;
+          powers(pc, at + j < vis ? fmaxf(zof(d[j]) - tau, 0.0f) : 0.0f, e, pa, pa1);
+          F += pa;
+          F1 += pa1;
+        }
       }
       F = wave_sum(F);
       F1 = wave_sum(F1);
@@ -420,65 +510,70 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
     }
   }
 
-  // ---- tau over the team's lists; every wave does the same steps ----
+  // ---- tau over the list, by every wave alike ----
+  float total = 0.0f;
   if (listed) {
     tau = lo;
-    for (int it = 0; it < kMaxSteps; ++it) {
+    bool done = false;
+    for (int it = 0; it <= kMaxSteps; ++it) {
       float F = 0.0f, F1 = 0.0f;
-      for (int i = 0; i < size; ++i) {
-        const float* z = L.lz + (w0 + i) * L.cap;
-        const int n = L.cnt[w0 + i];
-        for (int j = lane; j < n; j += kWave) {
-          float pa, pa1;
-          powers(pc, fmaxf(z[j] - tau, 0.0f), e, pa, pa1);
-          F += pa;
-          F1 += pa1;
-        }
+#pragma unroll 4
+      for (int j = lane; j < n; j += kWave) {
+        float pa, pa1;
+        powers(pc, fmaxf(lz[j] - tau, 0.0f), e, pa, pa1);
+        F += pa;
+        F1 += pa1;
       }
-      if (next_tau(p.alpha, wave_sum(F), wave_sum(F1), tau, lo, hi)) break;
+      total = wave_sum(F);
+      if (done || it == kMaxSteps) break;  // the sum at the final tau
+      done = next_tau(p.alpha, total, wave_sum(F1), tau, lo, hi);
     }
   }
-  __syncthreads();  // every wave has read the lists that their owners now reuse
+  __syncthreads();  // the list's parts may be overwritten
+  const int part = listed ? (n + size - 1) / size : 0, first = min(n, member * part);
+  const int m = listed ? min(part, n - first) : 0;
 
   // ---- the support's weights and values ----
   ValueSum<NG> vs;
   float psum = 0.0f;
+  float* pz = listed ? lz + first : L.lz + w * CAP;
+  int* pi = listed ? li + first : L.li + w * CAP;
   if (!empty) {
-    // listed: the wave's own list; else its keys of the row, cap at a time
-    const int per = listed ? mine : L.cap;
+    // listed: the wave's part of the list; else its keys of the row, CAP at a time
     const int end = listed ? 1 : vis;
-    for (int k0 = listed ? 0 : member * per; k0 < end; k0 += size * per) {
-      const int cnt = listed ? mine : min(per, vis - k0);
-      int n = 0;
+    for (int k0 = listed ? 0 : member * CAP; k0 < end; k0 += size * CAP) {
+      const int cnt = listed ? m : min(CAP, vis - k0);
+      int c = 0;
       for (int j0 = 0; j0 < cnt; j0 += kWave) {
         const int j = j0 + lane;
-        const float z = j >= cnt ? kHidden : listed ? lz[j] : zp[k0 + j];
-        const int key = j >= cnt ? 0 : listed ? li[j] : k0 + j;
+        const float zj = j >= cnt ? kHidden : listed ? pz[j] : zof(sp[k0 + j]);
+        const int key = j >= cnt ? 0 : listed ? pi[j] : k0 + j;
         float pa, pa1;
-        powers(pc, fmaxf(z - tau, 0.0f), e, pa, pa1);
-        const uint64_t m = __ballot(pa > 0.0f);
+        powers(pc, fmaxf(zj - tau, 0.0f), e, pa, pa1);
+        const uint64_t msk = __ballot(pa > 0.0f);
         if (pa > 0.0f) {
-          const int at = n + lane_rank(m);  // at most j: already read
-          lz[at] = pa;
-          li[at] = key;
+          const int at = c + lane_rank(msk);  // at most j: already read
+          pz[at] = pa;
+          pi[at] = key;
         }
-        n += __builtin_popcountll(m);
+        c += __builtin_popcountll(msk);
         psum += pa;
       }
-      vs.add(p, b, h, lz, li, n, lane);
+      vs.add(p, b, h, pz, pi, c, lane);
       if (listed) break;
     }
-    psum = wave_sum(psum);
   }
   vs.reduce();
-  constexpr int kCl = ValueSum<NG>::kCl;
-  if (lane < kCl && lane < 4 * NG)
+  if (lane < ValueSum<NG>::kCl && lane < 4 * NG)
     for (int j = 0; j < 8; ++j) L.acc[w * kAccStride + 8 * lane + j] = vs.acc[j];
-  if (lane == 0) L.red[4 * w + 3] = psum;
+  if (!listed) {
+    psum = wave_sum(psum);
+    if (lane == 0) L.red[4 * w + 3] = psum;
+  }
   __syncthreads();
   if (row >= 0) {
-    float total = 0.0f;
-    for (int i = 0; i < size; ++i) total += L.red[4 * (w0 + i) + 3];
+    if (!listed)
+      for (int i = 0; i < size; ++i) total += L.red[4 * (w0 + i) + 3];
     const float inv = total > 0.0f ? 1.0f / total : 0.0f;
     const int head = h * p.rep + row / p.NQ, i = row % p.NQ;
     T* out = static_cast<T*>(p.out) + ((size_t(b) * p.H + head) * p.NQ + i) * p.c.hd;
@@ -494,102 +589,91 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
 // Kernels
 // ---------------------------------------------------------------------------
 
-constexpr int kOneWaves = 16;   // one-block plan
-constexpr int kScoreWaves = 4;  // split plan: score blocks
+constexpr int kOneWaves = 8, kOneCap = 128;  // one-block plan
+constexpr int kScoreWaves = 4;               // split plan: score blocks
+constexpr int kRowKeys = 8192;               // rows up to this: 4 waves, else 16
 
-// One block per 16 rows of a key head: scores into LDS, then its rows.
-template <typename T, int NT, int NG>
-__global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnParams p, int cap, int stride) {
+// One block per tile of rows of a key head: dots into LDS, then its rows.
+template <typename T, int P, int NG>
+__global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnParams p, int stride) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
-  const int nrt = (p.R + kRows - 1) / kRows;
+  constexpr int kR = kTile / P;
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63, o = lane >> 4;
+  const int nrt = (p.R + kR - 1) / kR;
   const int rt = blockIdx.x % nrt, bh = blockIdx.x / nrt;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
-  const int r0 = rt * kRows, rows = min(kRows, p.R - r0);
-  const TeamLds L = team_lds<kOneWaves>(smem, cap);
-  float* zs = reinterpret_cast<float*>(smem + team_lds_bytes<kOneWaves>(cap));
-  int* pages = reinterpret_cast<int*>(zs + rows * stride);
-
+  const int r0 = rt * kR, rows = min(kR, p.R - r0);
+  float* zs = reinterpret_cast<float*>(smem);
+  const TeamLds L = team_lds<kOneWaves, kOneCap>(zs + min(kR, p.R) * stride);
+  int* pages = reinterpret_cast<int*>(L.acc + kOneWaves * kAccStride);
   const int len = max(0, min(p.lengths[b], p.maxlen));
   stage_pages(p, b, 0, len, pages, t, kOneWaves * kWave);
-  QueryFrag<T, NT, NG> q;
-  q.load(p, b, h, r0, lane);
-  __syncthreads();
-  const int o = lane >> 4;
-  score_keys<2, kOneWaves>(p, q, h, 0, len, pages, w, lane, [&](int r, int key, float z) {
-    if (4 * o + r < rows) zs[(4 * o + r) * stride + key] = z;
-  });
+  {
+    QueryFrag<T, P, NG> q;
+    q.load(p, b, h, r0, lane);
+    __syncthreads();
+    score_keys<P == 1 ? 2 : 1, kOneWaves>(p, q, h, 0, min(len, q.most), pages, w, lane, [&](int key, f32x4 d) {
+      for (int k = 0; k < 4; ++k) {
+        const int r = (4 * o + k) % kR;
+        if (r < rows) zs[r * stride + key] = d[k];
+      }
+    });
+  }
   __syncthreads();
   int pad = 1;
-  while (pad < rows) pad *= 2;
-  const int size = kOneWaves / pad, row = w / size, w0 = row * size;
-  const bool has = row < rows;
-  const int vis = has ? visible_keys(p, b, (r0 + row) % p.NQ) : 0;
-  const float* zp = zs + (has ? row : 0) * stride;
-  float zpart = kHidden;
-  for (int j = (w - w0) * kWave + lane; j < vis; j += size * kWave) zpart = fmaxf(zpart, zp[j]);
-  finish_row<T, NG, kOneWaves>(p, b, h, has ? r0 + row : -1, vis, zp, zpart, L, w, w0, size, lane);
+  while (pad < rows && pad < kOneWaves) pad *= 2;
+  const int size = kOneWaves / pad, team = w / size, w0 = team * size;
+  for (int first = 0; first < rows; first += pad) {
+    const int r = first + team;
+    const bool has = r < rows;
+    finish_row<T, NG, kOneWaves, kOneCap>(p, b, h, has ? r0 + r : -1, has ? visible_keys(p, b, (r0 + r) % p.NQ) : 0,
+                                          zs + (has ? r : 0) * stride, L, w, w0, size, lane);
+  }
 }
 
-// Split plan, first launch: z of `span` keys x 16 rows, and its maxima.
-template <typename T, int NT, int NG>
+// Split plan, first launch: dots of `span` keys with a tile of rows.
+template <typename T, int P, int NG>
 __global__ __launch_bounds__(kScoreWaves * kWave) void cache_score_kernel(CacheAttnParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ float wmax[kScoreWaves][kRows];
+  constexpr int kR = kTile / P;
   int* pages = reinterpret_cast<int*>(smem);
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, o = lane >> 4;
-  const int nrt = (p.R + kRows - 1) / kRows;
+  const int nrt = (p.R + kR - 1) / kR;
   const int split = blockIdx.x % p.nsplit, rest = blockIdx.x / p.nsplit;
   const int rt = rest % nrt, bh = rest / nrt;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
-  const int r0 = rt * kRows;
+  const int r0 = rt * kR;
   const int key0 = split * p.span;
   const int len = max(0, min(p.lengths[b], p.maxlen));
   if (key0 >= len) return;
   const int key1 = min(len, key0 + p.span);
   stage_pages(p, b, key0, key1 - key0, pages, t, kScoreWaves * kWave);
-  QueryFrag<T, NT, NG> q;
+  QueryFrag<T, P, NG> q;
   q.load(p, b, h, r0, lane);
   __syncthreads();
-  const size_t zstride = size_t(p.span) * p.nsplit;
-  float* zrow = p.scores + (size_t(bh) * p.R + r0 + 4 * o) * zstride;
-  float rmax[4] = {kHidden, kHidden, kHidden, kHidden};
-  const int nr = p.R - r0 - 4 * o;  // the lane's rows below nr are real
-  score_keys<4, kScoreWaves>(p, q, h, key0, key1, pages, w, lane, [&](int r, int key, float z) {
-    if (r < nr && key < key1) zrow[size_t(r) * zstride + key] = z;
-    rmax[r] = fmaxf(rmax[r], z);
-  });
-  for (int r = 0; r < 4; ++r) {
-    float m = rmax[r];
-    m = fmaxf(m, __uint_as_float(lane_xor<1>(__float_as_uint(m))));
-    m = fmaxf(m, __uint_as_float(lane_xor<2>(__float_as_uint(m))));
-    m = fmaxf(m, __uint_as_float(lane_xor<7>(__float_as_uint(m))));
-    m = fmaxf(m, __uint_as_float(lane_xor<15>(__float_as_uint(m))));
-    if ((lane & 15) == 0) wmax[w][4 * o + r] = m;
-  }
-  __syncthreads();
-  if (t < kRows && r0 + t < p.R) {
-    float m = wmax[0][t];
-    for (int i = 1; i < kScoreWaves; ++i) m = fmaxf(m, wmax[i][t]);
-    p.smax[(size_t(bh) * p.R + r0 + t) * p.nsplit + split] = m;
-  }
+  const size_t stride = size_t(p.span) * p.nsplit;
+  float* base = p.scores + (size_t(bh) * p.R + r0) * stride;
+  score_keys<P == 1 ? 4 : P == 2 ? 2 : 1, kScoreWaves>(
+      p, q, h, key0, min(key1, q.most), pages, w, lane, [&](int key, f32x4 d) {
+        if (key < key1)
+          for (int k = 0; k < 4; ++k) {
+            const int r = (4 * o + k) % kR;
+            if (r0 + r < p.R) base[size_t(r) * stride + key] = d[k];
+          }
+      });
 }
 
 // Split plan, second launch: one block per row.
 template <typename T, int NG, int NW>
-__global__ __launch_bounds__(NW * kWave) void cache_row_kernel(CacheAttnParams p, int cap) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+__global__ __launch_bounds__(NW * kWave) void cache_row_kernel(CacheAttnParams p) {
+  constexpr int kCap = 1024 / NW;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[team_lds_bytes<NW, kCap>()];
   const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   const int row = blockIdx.x % p.R, bh = blockIdx.x / p.R;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
-  const TeamLds L = team_lds<NW>(smem, cap);
-  const int vis = visible_keys(p, b, row % p.NQ);
-  const size_t at = size_t(bh) * p.R + row;
-  const float* zp = p.scores + at * (size_t(p.span) * p.nsplit);
-  const int ns = (vis + p.span - 1) / p.span;
-  float zpart = kHidden;
-  for (int j = t; j < ns; j += NW * kWave) zpart = fmaxf(zpart, p.smax[at * p.nsplit + j]);
-  finish_row<T, NG, NW>(p, b, h, row, vis, zp, zpart, L, w, 0, NW, lane);
+  const float* sp = p.scores + (size_t(bh) * p.R + row) * (size_t(p.span) * p.nsplit);
+  finish_row<T, NG, NW, kCap>(p, b, h, row, visible_keys(p, b, row % p.NQ), sp, team_lds<NW, kCap>(smem), w, 0, NW,
+                              lane);
 }
 
 template <typename K> hipError_t allow_lds(K kern, size_t lds) {
@@ -598,66 +682,79 @@ template <typename K> hipError_t allow_lds(K kern, size_t lds) {
                              int(lds));
 }
 
-constexpr int kOneCap = 256;   // candidates per wave, one-block plan
-constexpr int kRowCap = 512;   // candidates per wave, split plan
-constexpr int kRowWaves = 16;
+// Key tiles that share a result: as many as leave room for the rows.  fp32
+// queries (three terms) would need P times their 48 operand registers.
+int tiles_shared(const CacheAttnParams& p, int dtype) {
+  return dtype == kElemF32 || p.R > 8 ? 1 : p.R > 4 ? 2 : 4;
+}
 
-size_t one_lds_bytes(const CacheAttnParams& p, int* stride) {
-  const int rows = p.R < kRows ? p.R : kRows;
-  *stride = (p.maxlen + 15) / 16 * 16 + 4;
-  return team_lds_bytes<kOneWaves>(kOneCap) + size_t(rows) * *stride * 4 +
+size_t one_lds_bytes(const CacheAttnParams& p, int tile_rows, int* stride) {
+  const int rows = p.R < tile_rows ? p.R : tile_rows;
+  *stride = (p.maxlen + 63) / 64 * 64 + 4;
+  return team_lds_bytes<kOneWaves, kOneCap>() + size_t(rows) * *stride * 4 +
          size_t((p.maxlen + p.c.page - 1) / p.c.page + 1) * 4;
 }
 
-template <typename T, int NT, int NG>
-hipError_t launch_ng(const CacheAttnParams& p, hipStream_t s) {
-  const int nrt = (p.R + kRows - 1) / kRows;
+template <typename T, int P, int NG>
+hipError_t launch_png(const CacheAttnParams& p, hipStream_t s) {
+  const int nrt = (p.R + kTile / P - 1) / (kTile / P);
   if (p.plan == kCacheOneBlock) {
     int stride = 0;
-    const size_t lds = one_lds_bytes(p, &stride);
-    auto kern = cache_one_kernel<T, NT, NG>;
+    const size_t lds = one_lds_bytes(p, kTile / P, &stride);
+    auto kern = cache_one_kernel<T, P, NG>;
     if (hipError_t e = allow_lds(kern, lds)) return e;
     profile_begin("cache_attn", s);
-    hipLaunchKernelGGL(kern, dim3(unsigned(p.B) * p.c.heads * nrt), dim3(kOneWaves * kWave), lds, s, p, kOneCap,
-                       stride);
+    hipLaunchKernelGGL(kern, dim3(unsigned(p.B) * p.c.heads * nrt), dim3(kOneWaves * kWave), lds, s, p, stride);
     profile_end(s);
     return hipGetLastError();
   }
   profile_begin("cache_score", s);
-  hipLaunchKernelGGL((cache_score_kernel<T, NT, NG>), dim3(unsigned(p.B) * p.c.heads * nrt * p.nsplit),
+  hipLaunchKernelGGL((cache_score_kernel<T, P, NG>), dim3(unsigned(p.B) * p.c.heads * nrt * p.nsplit),
                      dim3(kScoreWaves * kWave), size_t(p.span / p.c.page + 1) * 4, s, p);
-  profile_end(s);
-  if (hipError_t e = hipGetLastError()) return e;
-  const size_t lds = team_lds_bytes<kRowWaves>(kRowCap);
-  auto kern = cache_row_kernel<T, NG, kRowWaves>;
-  if (hipError_t e = allow_lds(kern, lds)) return e;
-  profile_begin("cache_row", s);
-  hipLaunchKernelGGL(kern, dim3(unsigned(p.B) * p.c.heads * p.R), dim3(kRowWaves * kWave), lds, s, p, kRowCap);
   profile_end(s);
   return hipGetLastError();
 }
 
-template <typename T, int NT>
-hipError_t launch_t(const CacheAttnParams& p, hipStream_t s) {
+template <typename T, int NG>
+hipError_t launch_ng(const CacheAttnParams& p, int dtype, hipStream_t s) {
+  hipError_t e = hipSuccess;
+  if constexpr (std::is_same<T, float>::value) {
+    e = launch_png<T, 1, NG>(p, s);
+  } else {
+    const int P = tiles_shared(p, dtype);
+    e = P == 1 ? launch_png<T, 1, NG>(p, s) : P == 2 ? launch_png<T, 2, NG>(p, s) : launch_png<T, 4, NG>(p, s);
+  }
+  if (e != hipSuccess || p.plan == kCacheOneBlock) return e;
+  const dim3 grid(unsigned(p.B) * p.c.heads * p.R);
+  profile_begin("cache_row", s);
+  if (p.maxlen <= kRowKeys) hipLaunchKernelGGL((cache_row_kernel<T, NG, 4>), grid, dim3(4 * kWave), 0, s, p);
+  else hipLaunchKernelGGL((cache_row_kernel<T, NG, 16>), grid, dim3(16 * kWave), 0, s, p);
+  profile_end(s);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_t(const CacheAttnParams& p, int dtype, hipStream_t s) {
   switch (p.c.G) {
-    case 1: return launch_ng<T, NT, 1>(p, s);
-    case 2: return launch_ng<T, NT, 2>(p, s);
-    case 3: return launch_ng<T, NT, 3>(p, s);
-    default: return launch_ng<T, NT, 4>(p, s);
+    case 1: return launch_ng<T, 1>(p, dtype, s);
+    case 2: return launch_ng<T, 2>(p, dtype, s);
+    case 3: return launch_ng<T, 3>(p, dtype, s);
+    default: return launch_ng<T, 4>(p, dtype, s);
   }
 }
 
 }  // namespace
 
-size_t cache_attn_plan(CacheAttnParams& p, size_t max_lds, int cus) {
+size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus) {
+  const int tile_rows = kTile / tiles_shared(p, dtype);
   int stride = 0;
   p.span = p.nsplit = 0;
-  if (p.maxlen <= 2048 && one_lds_bytes(p, &stride) <= max_lds) {
+  if (p.maxlen <= 2048 && one_lds_bytes(p, tile_rows, &stride) <= max_lds) {
     p.plan = kCacheOneBlock;
     return 0;
   }
   p.plan = kCacheSplit;
-  const long long nrt = (p.R + kRows - 1) / kRows, tiles = (long long)p.B * p.c.heads * nrt;
+  const long long nrt = (p.R + tile_rows - 1) / tile_rows, tiles = (long long)p.B * p.c.heads * nrt;
   // eight score blocks per compute unit, of at least 256 keys (the largest
   // page: a block starts on a page)
   long long span = (p.maxlen * tiles + 8LL * cus - 1) / (8LL * cus);
@@ -665,14 +762,13 @@ size_t cache_attn_plan(CacheAttnParams& p, size_t max_lds, int cus) {
   if (span > 4096) span = 4096;
   p.span = int(span);
   p.nsplit = int((p.maxlen + span - 1) / span);
-  const size_t rows = size_t(p.B) * p.c.heads * p.R;
-  return rows * p.nsplit * (size_t(p.span) + 1) * sizeof(float);
+  return size_t(p.B) * p.c.heads * p.R * p.nsplit * size_t(p.span) * sizeof(float);
 }
 
 hipError_t launch_cache_attn(const CacheAttnParams& p, int dtype, hipStream_t s) {
-  if (dtype == kElemBF16) return launch_t<u16, 1>(p, s);
-  if (dtype == kElemF16) return launch_t<h16, 2>(p, s);
-  return launch_t<float, 3>(p, s);
+  if (dtype == kElemBF16) return launch_t<u16>(p, dtype, s);
+  if (dtype == kElemF16) return launch_t<h16>(p, dtype, s);
+  return launch_t<float>(p, dtype, s);
 }
 
 }  // namespace asa

@@ -425,7 +425,7 @@ int validate_query(const asa_cache* c, const asa_cache_query* a, bool pointers,
 }
 
 // Chooses how the call runs on the current device; its workspace bytes.
-int plan_query(asa::CacheAttnParams* ap, size_t* bytes) {
+int plan_query(asa::CacheAttnParams* ap, int dtype, size_t* bytes) {
   int dev = 0, max_lds = 0, cus = 0;
   if (int rc = check_hip(hipGetDevice(&dev), "hipGetDevice")) return rc;
   if (int rc = check_hip(hipDeviceGetAttribute(&max_lds, hipDeviceAttributeMaxSharedMemoryPerBlock,
@@ -433,9 +433,9 @@ int plan_query(asa::CacheAttnParams* ap, size_t* bytes) {
                          "hipDeviceGetAttribute"))
     return rc;
   if (int rc = device_cus(&cus)) return rc;
-  *bytes = asa::cache_attn_plan(*ap, size_t(max_lds), cus);
+  *bytes = asa::cache_attn_plan(*ap, dtype, size_t(max_lds), cus);
   const long long blocks = (long long)ap->B * ap->c.heads * ((ap->R + 15) / 16) *
-                           (ap->nsplit > 1 ? ap->nsplit : 1);
+                           (ap->nsplit > 1 ? ap->nsplit : 1);  // at least the launches' grids
   if (blocks >= (1LL << 31)) return fail(ASA_ERR_INVALID_ARGUMENT, "problem too large");
   return ASA_OK;
 }
@@ -890,7 +890,7 @@ int asa_cache_attention_workspace(const asa_cache* c, const asa_cache_query* a, 
   asa::CacheAttnParams ap{};
   if (int rc = validate_query(c, a, false, &ap)) return rc;
   if (!bytes) return fail(ASA_ERR_INVALID_ARGUMENT, "an argument is NULL");
-  if (int rc = plan_query(&ap, bytes)) return rc;
+  if (int rc = plan_query(&ap, a->dtype, bytes)) return rc;
   return ok();
 }
 
@@ -900,14 +900,13 @@ int asa_cache_attention(const asa_cache* c, const asa_cache_query* a, const void
   if (int rc = validate_query(c, a, true, &ap)) return rc;
   if (!q || !out) return fail(ASA_ERR_INVALID_ARGUMENT, "a tensor argument is NULL");
   size_t bytes = 0;
-  if (int rc = plan_query(&ap, &bytes)) return rc;
+  if (int rc = plan_query(&ap, a->dtype, &bytes)) return rc;
   if (bytes && !workspace) return fail(ASA_ERR_INVALID_ARGUMENT, "workspace is NULL");
   if (int rc = check_aligned({workspace})) return rc;
   ap.q = q;
   ap.chunks = whole_chunks(q, ap.lq, c->head_dim, a->dtype);
   ap.out = out;
   ap.scores = static_cast<float*>(workspace);
-  ap.smax = ap.scores + size_t(ap.B) * ap.c.heads * ap.R * ap.span * ap.nsplit;
   if (int rc = check_hip(asa::launch_cache_attn(ap, a->dtype, static_cast<hipStream_t>(stream)),
                          "cache attention kernel launch"))
     return rc;

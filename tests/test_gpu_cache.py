@@ -225,7 +225,7 @@ def check_attention(out, q, k, v, lengths, q_idx, alpha, scale, what=""):
                 assert not bool(out[b, h].any()), what
                 continue
             s = (kk.amax() - kk.amin()) / 15
-            dz = (alpha - 1) * (scale * 10 * 2.0 ** -24 * 30 * float(s) * math.sqrt(d / 32)
+            dz = (alpha - 1) * (abs(scale) * 10 * 2.0 ** -24 * 30 * float(s) * math.sqrt(d / 32)
                                 * q64[b, h].norm(dim=1) + 10 * 2.0 ** -24)
             tol = (4 * sens * dz + 2.0 ** -17) * float(vv.abs().amax())
             got = out[b, h].double().cpu()
@@ -257,6 +257,7 @@ SHAPES = [
     ([3001], 1, 9, 3, 128, 16),
     ([5000, 4999], 1, 1, 1, 100, 256),
     ([9000], 1, 2, 1, 33, 128),
+    ([70001], 1, 2, 1, 32, 64),
 ]
 
 
@@ -294,6 +295,16 @@ def test_flat_and_peaked_rows(dev, n, qscale, alpha):
     q = torch.randn(1, 2, 1, 64, generator=torch.Generator().manual_seed(8)) * qscale
     out = c.attention(q.to(dev), table, L, alpha=alpha)
     check_attention(out, q, k, v, [n], [[n - 1]], alpha, 0.125)
+
+
+@pytest.mark.parametrize("n", [150, 2500])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_scales_of_any_sign(dev, n, scale):
+    c, table, L, k, v = filled(dev, [n], 2, 64, 32, torch.bfloat16, 20)
+    for rep in (1, 3, 6, 10):  # each number of key tiles that share a result
+        q = torch.randn(1, 2 * rep, 1, 64, generator=torch.Generator().manual_seed(rep)).bfloat16()
+        out = c.attention(q.to(dev), table, L, sm_scale=scale)
+        check_attention(out, q, k, v, [n], [[n - 1]], 1.5, scale)
 
 
 @pytest.mark.parametrize("n", [100, 3000])
