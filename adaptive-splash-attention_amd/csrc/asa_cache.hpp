@@ -81,9 +81,12 @@ struct CacheAttnParams {
   bool chunks;            // as above, for q
   void* out;              // [B, H, NQ, hd] contiguous
   float alpha, scale;
+  float e, zc, zb;        // 1 / (alpha - 1), (alpha - 1) |scale|, 10 (alpha - 1)
+  int pc;                 // pow_class_of(e)
   int plan;               // CachePlan
   int span, nsplit;       // split plan: keys per score block, score blocks per row tile
-  float* scores;          // split plan: [B * c.heads * R, span * nsplit]
+  float* scores;          // split plan: dots, [B * c.heads * R, span * nsplit]
+  float* gmax;            // split plan: each 64 keys' maxima, [B * c.heads * R, span * nsplit / 64]
 };
 // How attention runs: one block per 16 rows that holds their scores in LDS,
 // or the keys split over score blocks, then one block per row.

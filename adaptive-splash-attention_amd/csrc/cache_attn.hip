@@ -20,11 +20,15 @@
 // type.
 //
 // tau lies in [max z - 1, max z], so only keys with z > max z - 1 can have a
-// weight.  A row's z are held in registers, the candidates are listed (index,
-// z) in LDS, Newton steps over the list find tau, and only the value rows of
-// the support are read, by their entry in the list.  alpha-entmax gives most
-// keys of a long row no weight, so the values' bytes are a small part of the
-// keys'.  Lists have a fixed order, so results do not depend on timing.
+// weight.  A better bound: the sum over any part of the row is at most the
+// whole one, so the tau of the row's granule maxima (the largest z of each 64
+// keys, which the score pass keeps) is at most tau, and close to it, since a
+// long row's support lies in as many granules.  Only granules whose maximum
+// is above that bound are looked at again: their keys above it are listed
+// (index, z) in LDS, Newton steps over the list find tau, and only the value
+// rows of the support are read.  alpha-entmax gives most keys of a long row
+// no weight, so the values' bytes are a small part of the keys'.  Lists have
+// a fixed order, so results do not depend on timing.
 #include <climits>
 #include <type_traits>
 
@@ -34,7 +38,8 @@
 namespace asa {
 namespace {
 
-constexpr float kHidden = -3e38f;  // score of a key that a row does not see
+constexpr float kHidden = -3e38f;     // dot and z of a key that a row does not see
+constexpr float kNotNumber = -1e38f;  // a dot that is not a number: the score clamp makes it -10
 constexpr int kTile = 16;          // rows and keys of an MFMA tile
 
 // ---------------------------------------------------------------------------
@@ -189,14 +194,12 @@ __device__ __forceinline__ f32x4 dots(const QueryFrag<T, P, NG>& q, const KeyPac
   return s;
 }
 
-// z = (alpha - 1) clamp(|scale| dot), hidden keys apart; a dot that is not a
-// number counts as the lower bound, as in the score clamp of the dense path.
+// z = (alpha - 1) clamp(|scale| dot), hidden keys apart.
 struct ZOf {
   float c, zb;
-  __device__ __forceinline__ explicit ZOf(const CacheAttnParams& p)
-      : c((p.alpha - 1.0f) * fabsf(p.scale)), zb(10.0f * (p.alpha - 1.0f)) {}
+  __device__ __forceinline__ explicit ZOf(const CacheAttnParams& p) : c(p.zc), zb(p.zb) {}
   __device__ __forceinline__ float operator()(float dot) const {
-    return dot == kHidden ? kHidden : __builtin_amdgcn_fmed3f(dot * c, -zb, zb);
+    return dot <= 2.0f * kNotNumber ? kHidden : __builtin_amdgcn_fmed3f(dot * c, -zb, zb);
   }
 };
 
@@ -211,37 +214,62 @@ __device__ __forceinline__ void stage_pages(const CacheAttnParams& p, int b, int
   }
 }
 
-// Dots of the keys [key0, key1) by the block's NW waves, V packs per wave in
-// flight, handed to put(key, dots) (dots as from `dots`; hidden where a row
-// does not see the key).  key0 is a multiple of the page size.
-template <int V, int NW, typename T, int P, int NG, typename Put>
+// Dots of the keys [key0, key1) by the block's NW waves, a granule of 64 keys
+// per wave and step (4 / P packs; the next step's loads are in flight
+// meanwhile), handed to put(key, dots) (dots as from `dots`; hidden where a
+// row does not see the key); the granule's maxima of each row to
+// most(granule, row of the tile, maximum) by one lane.  key0 is a multiple of
+// the page size and of 64.
+constexpr int kGranule = 64;
+template <int NW, typename T, int P, int NG, typename Put, typename Most>
 __device__ __forceinline__ void score_keys(const CacheAttnParams& p, const QueryFrag<T, P, NG>& q, int h,
                                            int key0, int key1, const int* pages, int w, int lane,
-                                           Put put) {
-  constexpr int kKeys = kTile * P, kStep = NW * V * kKeys;
+                                           Put put, Most most) {
+  constexpr int V = 4 / P, kKeys = kTile * P, kR = kTile / P;
   const int own = kTile * ((lane >> 4) * P / 4) + (lane & 15);
   KeyPack<P, NG> next[V];
-  int base = key0 + w * (V * kKeys);
+  int base = key0 + w * kGranule;
   if (base < key1)
 #pragma unroll
     for (int v = 0; v < V; ++v) next[v].load(p.c, h, pages, key0, base + v * kKeys, key1, lane);
-  for (; base < key1; base += kStep) {
+  for (; base < key1; base += NW * kGranule) {
     KeyPack<P, NG> k[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) k[v] = next[v];
-    if (base + kStep < key1)
+    const int ahead = base + NW * kGranule;
+    if (ahead < key1)
 #pragma unroll
-      for (int v = 0; v < V; ++v) next[v].load(p.c, h, pages, key0, base + kStep + v * kKeys, key1, lane);
+      for (int v = 0; v < V; ++v) next[v].load(p.c, h, pages, key0, ahead + v * kKeys, key1, lane);
+    f32x4 m = {kHidden, kHidden, kHidden, kHidden};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int first = base + v * kKeys, key = first + own;
       if (first < key1) {
         f32x4 d = dots<T, P, NG>(q, k[v]);
+        for (int r = 0; r < 4; ++r) d[r] = fmaxf(d[r], kNotNumber);
         if (first + kKeys > q.least)
           for (int r = 0; r < 4; ++r) d[r] = key < q.vis[r] ? d[r] : kHidden;
         for (int r = 0; r < 4; ++r) d[r] = k[v].seen ? d[r] : kHidden;
         put(key, d);
+        for (int r = 0; r < 4; ++r) m[r] = fmaxf(m[r], d[r]);
       }
+    }
+    for (int r = 0; r < 4; ++r) {
+      float x = m[r];
+      x = fmaxf(x, __uint_as_float(lane_xor<1>(__float_as_uint(x))));
+      x = fmaxf(x, __uint_as_float(lane_xor<2>(__float_as_uint(x))));
+      x = fmaxf(x, __uint_as_float(lane_xor<7>(__float_as_uint(x))));
+      x = fmaxf(x, __uint_as_float(lane_xor<15>(__float_as_uint(x))));
+      if constexpr (P >= 2) {
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+      }
+      if constexpr (P == 4) {
+        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+      }
+      const int row = 4 * (lane >> 4) + r;
+      if ((lane & 15) == 0 && row < kR) most(base / kGranule, row, x);
     }
   }
 }
@@ -265,17 +293,6 @@ __device__ __forceinline__ float wave_sum(float v) {
 __device__ __forceinline__ float wave_max(float v) {
   return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
-// Sum over the lanes up to and with the calling one.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return v;
-}
-
 // v^e and v^(e-1), v >= 0, both 0 at v = 0.
 __device__ __forceinline__ void powers(int pc, float v, float e, float& pa, float& pa1) {
   if (pc == kE2) {
@@ -313,28 +330,20 @@ __device__ __forceinline__ bool next_tau(float alpha, float F, float F1, float& 
 }
 constexpr int kMaxSteps = 64;
 
-// LDS of the row teams: each wave's share of its team's candidate list, and
-// partial results.
+// LDS of the row teams.  A wave collects up to CAP candidates of its row; a
+// list of up to kList is gathered for the whole team (8 registers of a wave).
+constexpr int kList = 512;
 constexpr int kAccStride = 132;
-struct TeamLds {
-  float* lz;   // [NW * cap] z, later p
-  int* li;     // [NW * cap] key
-  float* red;  // [NW][4]
-  int* cnt;    // [NW]
-  float* acc;  // [NW][kAccStride]
+template <int NW, int CAP> struct TeamLds {
+  static constexpr int kCap = CAP;
+  float cz[NW][CAP];  // a wave's candidates, later its part of the support
+  int ci[NW][CAP];
+  float gm[NW][kWave];
+  float red[2][NW][2];
+  float psum[NW];
+  int cnt[NW];
+  float acc[NW][kAccStride];
 };
-template <int NW, int CAP> constexpr size_t team_lds_bytes() {
-  return size_t(NW) * (size_t(CAP) * 8 + 16 + 4 + kAccStride * 4);
-}
-template <int NW, int CAP> __device__ __forceinline__ TeamLds team_lds(void* base) {
-  TeamLds l;
-  l.lz = static_cast<float*>(base);
-  l.li = reinterpret_cast<int*>(l.lz + NW * CAP);
-  l.red = reinterpret_cast<float*>(l.li + NW * CAP);
-  l.cnt = reinterpret_cast<int*>(l.red + NW * 4);
-  l.acc = reinterpret_cast<float*>(l.cnt + NW);
-  return l;
-}
 
 // Adds p_j v_j of the wave's listed keys to the lane's 8 channels: CL lanes
 // have a row's octets, so a step takes 64 / CL entries, four loads deep.
@@ -388,198 +397,244 @@ struct ValueSum {
 };
 
 // tau and the output of row `row` (of the key head's R) from its dots at
-// sp[0 .. vis) (16-byte aligned), by `size` waves of the block from wave w0
-// on.  Every wave of the block calls it together (teams meet at the block's
-// barriers); row = -1, vis = 0 for a team without a row.  A lane holds 32 z
-// at a time: rows of at most 2048 * size keys stay in registers, longer ones
-// are read again at each step.
-constexpr int kQuads = 8;  // 16-byte loads of a lane
-template <typename T, int NG, int NW, int CAP>
+// sp[0 .. vis) and their granule maxima gp, by `size` waves of the block from
+// wave w0 on; lz, li: kList entries of (z, key) of the team.  Every wave of
+// the block calls it together (teams meet at the block's barriers); row = -1,
+// vis = 0 for a team without a row.  WHOLE: the team is the block.
+template <typename T, int NG, int NW, bool WHOLE, typename Lds>
 __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int h, int row, int vis,
-                                           const float* sp, const TeamLds& L, int w, int w0, int size,
-                                           int lane) {
-  const int member = w - w0;
-  const float e = 1.0f / (p.alpha - 1.0f);
-  const int pc = pow_class_of(e);
+                                           const float* gp, const float* sp, Lds& L, float* lz, int* li, int w,
+                                           int w0, int size, int lane) {
+  constexpr int kCap = Lds::kCap;
+  const int member = w - w0, pc = p.pc;
+  const float e = p.e;
   const ZOf zof(p);
-  const int seg = size * kWave * 4 * kQuads;
-  const bool once = vis <= seg;
-  float z[4 * kQuads];
-  auto fetch = [&](int s0) {
-#pragma unroll
-    for (int q = 0; q < kQuads; ++q) {
-      const int at = s0 + ((q * size + member) * kWave + lane) * 4;
-      float4 f = float4{kHidden, kHidden, kHidden, kHidden};
-      if (at < vis) f = *reinterpret_cast<const float4*>(sp + at);
-      z[4 * q] = at < vis ? zof(f.x) : kHidden;
-      z[4 * q + 1] = at + 1 < vis ? zof(f.y) : kHidden;
-      z[4 * q + 2] = at + 2 < vis ? zof(f.z) : kHidden;
-      z[4 * q + 3] = at + 3 < vis ? zof(f.w) : kHidden;
-    }
-  };
-  // body(key of z[0], z) over the row's parts; z[4 q + j]: 256 size q + j further
-  auto sweep = [&](auto body) {
-    for (int s0 = 0; s0 < vis; s0 += seg) {
-      if (!once) fetch(s0);
-      body(s0 + (member * kWave + lane) * 4);
-    }
-  };
-  if (once) fetch(0);
-  float zpart = kHidden;
-  sweep([&](int) {
-#pragma unroll
-    for (int k = 0; k < 4 * kQuads; ++k) zpart = fmaxf(zpart, z[k]);
-  });
-  const float wm = wave_max(zpart);
-  if (lane == 0) L.red[4 * w] = wm;
+
+  // ---- the largest z, and a bound below tau from the granules' ----
+  const int ng = (vis + kGranule - 1) / kGranule;
+  float g = kHidden;
+#pragma unroll 4
+  for (int j = member * kWave + lane; j < ng; j += size * kWave) g = fmaxf(g, gp[j]);
+  L.gm[w][lane] = zof(g);
   __syncthreads();
-  float zmax = kHidden;
-  for (int i = 0; i < size; ++i) zmax = fmaxf(zmax, L.red[4 * (w0 + i)]);
+  float gz[4] = {kHidden, kHidden, kHidden, kHidden};
+  for (int i = 0; i < size; i += 4)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < size) gz[k] = fmaxf(gz[k], L.gm[w0 + i + k][lane]);
+  const float zmax = wave_max(fmaxf(fmaxf(gz[0], gz[1]), fmaxf(gz[2], gz[3])));
   const bool empty = !(zmax > 0.5f * kHidden);
   float tau = zmax - 1.0f, lo = tau, hi = zmax;
+  if (vis > kList && !empty) {
+    // a few steps: any tau left of the root of the maxima will do
+    for (int it = 0; it < 12; ++it) {
+      float F = 0.0f, F1 = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float pa, pa1;
+        powers(pc, fmaxf(gz[k] - tau, 0.0f), e, pa, pa1);
+        F += pa;
+        F1 += pa1;
+      }
+      F = wave_sum(F);
+      if (F < 1.01f && p.alpha <= 2.0f) break;
+      if (next_tau(p.alpha, F, wave_sum(F1), tau, lo, hi)) break;
+    }
+    // the rounding of the steps, and of F at them
+    if (p.alpha <= 2.0f) lo = tau;
+    lo = fmaxf(lo - 4e-6f, zmax - 1.0f);
+    tau = lo;
+    hi = zmax;
+  }
 
   // ---- the keys with z > lo, listed; lo moves up while they do not fit ----
-  float* lz = L.lz + w0 * CAP;
-  int* li = L.li + w0 * CAP;
-  bool listed = false, dense = empty;
-  int n = 0;
+  bool listed = false, big = false, dense = empty;
+  int n = 0, mine = 0;
   for (int it = 0;; ++it) {
-    int mine = 0, upto = 0;
     if (!listed && !dense) {
-      sweep([&](int) {
+      mine = 0;
+      auto collect = [&](float d, int key) {
+        const float z = key < vis ? zof(d) : kHidden;
+        const uint64_t m = __ballot(z > lo);
+        const int at = mine + lane_rank(m);
+        if (z > lo && at < kCap) {
+          L.cz[w][at] = z;
+          L.ci[w][at] = key;
+        }
+        mine += __builtin_popcountll(m);
+      };
+      // granule i is member i % size's
+      for (int i0 = 0; i0 < ng; i0 += size * kWave) {
+        const int i = i0 + lane * size + member;
+        uint64_t todo = __ballot(i < ng && zof(gp[i < ng ? i : 0]) > lo);
+        while (todo) {
+          float d[4];
+          int key[4];
 #pragma unroll
-        for (int k = 0; k < 4 * kQuads; ++k) mine += z[k] > lo ? 1 : 0;
-      });
-      upto = wave_scan(mine);
-      if (lane == kWave - 1) L.cnt[w] = upto;
+          for (int k = 0; k < 4; ++k) {
+            const int l = todo ? __builtin_ctzll(todo) : -1;
+            todo &= todo - 1;
+            key[k] = l < 0 ? vis : (i0 + l * size + member) * kGranule + lane;
+            d[k] = sp[key[k] < vis ? key[k] : 0];
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) collect(d[k], key[k]);
+        }
+      }
+      if (lane == 0) L.cnt[w] = mine;
     }
     __syncthreads();
     if (!listed && !dense) {
       n = 0;
       int before = 0;
+      bool fits = true;
       for (int i = 0; i < size; ++i) {
+        const int c = L.cnt[w0 + i];
         if (i == member) before = n;
-        n += L.cnt[w0 + i];
+        n += c;
+        fits = fits && c <= kCap;
       }
-      listed = n <= size * CAP;
-      if (listed) {
-        int at = before + upto - mine;
-        sweep([&](int key) {
-          if (mine)
-#pragma unroll
-            for (int k = 0; k < 4 * kQuads; ++k)
-              if (z[k] > lo) {
-                lz[at] = z[k];
-                li[at] = key + (k >> 2) * (size * kWave * 4) + (k & 3);
-                ++at;
-              }
-        });
-      }
+      listed = fits && (WHOLE || n <= kList);
+      big = listed && n > kList;
+      if (listed && !big)
+        for (int j = lane; j < mine; j += kWave) {
+          lz[before + j] = L.cz[w][j];
+          li[before + j] = L.ci[w][j];
+        }
     }
     if (!__syncthreads_or(!listed && !dense)) break;
     // some team's candidates did not fit: one step of its tau over the whole row
     float F = 0.0f, F1 = 0.0f;
     if (!listed && !dense) {
-#pragma unroll 2
-      for (int at = (member * kWave + lane) * 4; at < vis; at += size * kWave * 4) {
-        const float4 f = *reinterpret_cast<const float4*>(sp + at);
-        const float d[4] = {f.x, f.y, f.z, f.w};
-        for (int j = 0; j < 4; ++j) {
-          float pa, pa1;
-          powers(pc, at + j < vis ? fmaxf(zof(d[j]) - tau, 0.0f) : 0.0f, e, pa, pa1);
-          F += pa;
-          F1 += pa1;
-        }
+#pragma unroll 4
+      for (int j = member * kWave + lane; j < vis; j += size * kWave) {
+        float pa, pa1;
+        powers(pc, fmaxf(zof(sp[j]) - tau, 0.0f), e, pa, pa1);
+        F += pa;
+        F1 += pa1;
       }
       F = wave_sum(F);
       F1 = wave_sum(F1);
       if (lane == 0) {
-        L.red[4 * w + 1] = F;
-        L.red[4 * w + 2] = F1;
+        L.red[0][w][0] = F;
+        L.red[0][w][1] = F1;
       }
     }
     __syncthreads();
     if (!listed && !dense) {
       F = F1 = 0.0f;
       for (int i = 0; i < size; ++i) {
-        F += L.red[4 * (w0 + i) + 1];
-        F1 += L.red[4 * (w0 + i) + 2];
+        F += L.red[0][w0 + i][0];
+        F1 += L.red[0][w0 + i][1];
       }
       dense = next_tau(p.alpha, F, F1, tau, lo, hi) || it == kMaxSteps;
       if (p.alpha <= 2.0f) lo = tau;  // the steps stay left of the root
     }
   }
 
-  // ---- tau over the list, by every wave alike ----
+  // ---- tau over the list ----
   float total = 0.0f;
   if (listed) {
     tau = lo;
     bool done = false;
-    for (int it = 0; it <= kMaxSteps; ++it) {
-      float F = 0.0f, F1 = 0.0f;
-#pragma unroll 4
-      for (int j = lane; j < n; j += kWave) {
-        float pa, pa1;
-        powers(pc, fmaxf(lz[j] - tau, 0.0f), e, pa, pa1);
-        F += pa;
-        F1 += pa1;
+    if (!big) {  // in registers, by every wave alike
+      constexpr int kRegs = kList / kWave;
+      float z[kRegs];
+#pragma unroll
+      for (int k = 0; k < kRegs; ++k) z[k] = k * kWave + lane < n ? lz[k * kWave + lane] : kHidden;
+      for (int it = 0; it <= kMaxSteps; ++it) {
+        float F = 0.0f, F1 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRegs; ++k)
+          if (k * kWave < n) {
+            float pa, pa1;
+            powers(pc, fmaxf(z[k] - tau, 0.0f), e, pa, pa1);
+            F += pa;
+            F1 += pa1;
+          }
+        total = wave_sum(F);
+        if (done || it == kMaxSteps) break;  // the sum at the final tau
+        done = next_tau(p.alpha, total, wave_sum(F1), tau, lo, hi);
       }
-      total = wave_sum(F);
-      if (done || it == kMaxSteps) break;  // the sum at the final tau
-      done = next_tau(p.alpha, total, wave_sum(F1), tau, lo, hi);
+    } else {  // each wave its candidates; the block's barriers are the team's
+      for (int it = 0; it <= kMaxSteps; ++it) {
+        float F = 0.0f, F1 = 0.0f;
+#pragma unroll 2
+        for (int j = lane; j < mine; j += kWave) {
+          float pa, pa1;
+          powers(pc, fmaxf(L.cz[w][j] - tau, 0.0f), e, pa, pa1);
+          F += pa;
+          F1 += pa1;
+        }
+        F = wave_sum(F);
+        F1 = wave_sum(F1);
+        if (lane == 0) {
+          L.red[it & 1][w][0] = F;
+          L.red[it & 1][w][1] = F1;
+        }
+        __syncthreads();
+        total = F1 = 0.0f;
+        for (int i = 0; i < size; ++i) {
+          total += L.red[it & 1][i][0];
+          F1 += L.red[it & 1][i][1];
+        }
+        if (done || it == kMaxSteps) break;
+        done = next_tau(p.alpha, total, F1, tau, lo, hi);
+      }
     }
   }
-  __syncthreads();  // the list's parts may be overwritten
-  const int part = listed ? (n + size - 1) / size : 0, first = min(n, member * part);
-  const int m = listed ? min(part, n - first) : 0;
 
   // ---- the support's weights and values ----
   ValueSum<NG> vs;
   float psum = 0.0f;
-  float* pz = listed ? lz + first : L.lz + w * CAP;
-  int* pi = listed ? li + first : L.li + w * CAP;
   if (!empty) {
-    // listed: the wave's part of the list; else its keys of the row, CAP at a time
-    const int end = listed ? 1 : vis;
-    for (int k0 = listed ? 0 : member * CAP; k0 < end; k0 += size * CAP) {
-      const int cnt = listed ? m : min(CAP, vis - k0);
+    // the wave's part of the list, or its candidates, or its keys of the
+    // row, kCap at a time
+    const bool small = listed && !big;
+    const int part = small ? (n + size - 1) / size : big ? mine : kCap;
+    const int end = small ? min(n, (member + 1) * part) : big ? mine : vis;
+    for (int k0 = big ? 0 : member * part; k0 < end; k0 += size * part) {
+      const int cnt = min(part, end - k0);
       int c = 0;
       for (int j0 = 0; j0 < cnt; j0 += kWave) {
         const int j = j0 + lane;
-        const float zj = j >= cnt ? kHidden : listed ? pz[j] : zof(sp[k0 + j]);
-        const int key = j >= cnt ? 0 : listed ? pi[j] : k0 + j;
+        float zj = kHidden;
+        int key = 0;
+        if (j < cnt) {
+          zj = small ? lz[k0 + j] : big ? L.cz[w][j] : zof(sp[k0 + j]);
+          key = small ? li[k0 + j] : big ? L.ci[w][j] : k0 + j;
+        }
         float pa, pa1;
         powers(pc, fmaxf(zj - tau, 0.0f), e, pa, pa1);
         const uint64_t msk = __ballot(pa > 0.0f);
         if (pa > 0.0f) {
           const int at = c + lane_rank(msk);  // at most j: already read
-          pz[at] = pa;
-          pi[at] = key;
+          L.cz[w][at] = pa;
+          L.ci[w][at] = key;
         }
         c += __builtin_popcountll(msk);
         psum += pa;
       }
-      vs.add(p, b, h, pz, pi, c, lane);
-      if (listed) break;
+      vs.add(p, b, h, L.cz[w], L.ci[w], c, lane);
     }
   }
   vs.reduce();
   if (lane < ValueSum<NG>::kCl && lane < 4 * NG)
-    for (int j = 0; j < 8; ++j) L.acc[w * kAccStride + 8 * lane + j] = vs.acc[j];
+    for (int j = 0; j < 8; ++j) L.acc[w][8 * lane + j] = vs.acc[j];
   if (!listed) {
     psum = wave_sum(psum);
-    if (lane == 0) L.red[4 * w + 3] = psum;
+    if (lane == 0) L.psum[w] = psum;
   }
   __syncthreads();
   if (row >= 0) {
     if (!listed)
-      for (int i = 0; i < size; ++i) total += L.red[4 * (w0 + i) + 3];
+      for (int i = 0; i < size; ++i) total += L.psum[w0 + i];
     const float inv = total > 0.0f ? 1.0f / total : 0.0f;
     const int head = h * p.rep + row / p.NQ, i = row % p.NQ;
     T* out = static_cast<T*>(p.out) + ((size_t(b) * p.H + head) * p.NQ + i) * p.c.hd;
     for (int ch = member * kWave + lane; ch < p.c.hd; ch += size * kWave) {
       float v = 0.0f;
-      for (int k = 0; k < size; ++k) v += L.acc[(w0 + k) * kAccStride + ch];
+      for (int k = 0; k < size; ++k) v += L.acc[w0 + k][ch];
       Elem<T>::store(out + ch, v * inv);
     }
   }
@@ -589,49 +644,60 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
 // Kernels
 // ---------------------------------------------------------------------------
 
-constexpr int kOneWaves = 8, kOneCap = 128;  // one-block plan
-constexpr int kScoreWaves = 4;               // split plan: score blocks
-constexpr int kRowKeys = 8192;               // rows up to this: 4 waves, else 16
+constexpr int kOneWaves = 8;    // one-block plan
+constexpr int kScoreWaves = 4;  // split plan: score blocks
+constexpr int kRowKeys = 8192;  // split plan: rows up to this have 4 waves, else 16
 
 // One block per tile of rows of a key head: dots into LDS, then its rows.
+using OneLds = TeamLds<kOneWaves, 128>;
 template <typename T, int P, int NG>
 __global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnParams p, int stride) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ OneLds L;
   constexpr int kR = kTile / P;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, o = lane >> 4;
   const int nrt = (p.R + kR - 1) / kR;
   const int rt = blockIdx.x % nrt, bh = blockIdx.x / nrt;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
-  const int r0 = rt * kR, rows = min(kR, p.R - r0);
+  const int r0 = rt * kR, rows = min(kR, p.R - r0), most = min(kR, p.R), gs = stride / kGranule;
+  int pad = 1;
+  while (pad < most && pad < kOneWaves) pad *= 2;
   float* zs = reinterpret_cast<float*>(smem);
-  const TeamLds L = team_lds<kOneWaves, kOneCap>(zs + min(kR, p.R) * stride);
-  int* pages = reinterpret_cast<int*>(L.acc + kOneWaves * kAccStride);
+  float* gs0 = zs + most * stride;  // granule maxima
+  float* lz = gs0 + most * gs;      // a list for each of `pad` teams
+  int* li = reinterpret_cast<int*>(lz + pad * kList);
+  int* pages = li + pad * kList;
+  stage_pages(p, b, 0, p.maxlen, pages, t, kOneWaves * kWave);
   const int len = max(0, min(p.lengths[b], p.maxlen));
-  stage_pages(p, b, 0, len, pages, t, kOneWaves * kWave);
   {
     QueryFrag<T, P, NG> q;
     q.load(p, b, h, r0, lane);
     __syncthreads();
-    score_keys<P == 1 ? 2 : 1, kOneWaves>(p, q, h, 0, min(len, q.most), pages, w, lane, [&](int key, f32x4 d) {
-      for (int k = 0; k < 4; ++k) {
-        const int r = (4 * o + k) % kR;
-        if (r < rows) zs[r * stride + key] = d[k];
-      }
-    });
+    score_keys<kOneWaves>(
+        p, q, h, 0, min(len, q.most), pages, w, lane,
+        [&](int key, f32x4 d) {
+          for (int k = 0; k < 4; ++k) {
+            const int r = (4 * o + k) % kR;
+            if (r < rows) zs[r * stride + key] = d[k];
+          }
+        },
+        [&](int granule, int r, float m) {
+          if (r < rows) gs0[r * gs + granule] = m;
+        });
   }
   __syncthreads();
-  int pad = 1;
-  while (pad < rows && pad < kOneWaves) pad *= 2;
   const int size = kOneWaves / pad, team = w / size, w0 = team * size;
   for (int first = 0; first < rows; first += pad) {
     const int r = first + team;
     const bool has = r < rows;
-    finish_row<T, NG, kOneWaves, kOneCap>(p, b, h, has ? r0 + r : -1, has ? visible_keys(p, b, (r0 + r) % p.NQ) : 0,
-                                          zs + (has ? r : 0) * stride, L, w, w0, size, lane);
+    finish_row<T, NG, kOneWaves, false>(p, b, h, has ? r0 + r : -1, has ? visible_keys(p, b, (r0 + r) % p.NQ) : 0,
+                                        gs0 + (has ? r : 0) * gs, zs + (has ? r : 0) * stride, L, lz + team * kList,
+                                        li + team * kList, w, w0, size, lane);
   }
 }
 
-// Split plan, first launch: dots of `span` keys with a tile of rows.
+// Split plan, first launch: dots of `span` keys with a tile of rows, and
+// their granules' maxima.
 template <typename T, int P, int NG>
 __global__ __launch_bounds__(kScoreWaves * kWave) void cache_score_kernel(CacheAttnParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -651,29 +717,34 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void cache_score_kernel(CacheA
   QueryFrag<T, P, NG> q;
   q.load(p, b, h, r0, lane);
   __syncthreads();
-  const size_t stride = size_t(p.span) * p.nsplit;
-  float* base = p.scores + (size_t(bh) * p.R + r0) * stride;
-  score_keys<P == 1 ? 4 : P == 2 ? 2 : 1, kScoreWaves>(
-      p, q, h, key0, min(key1, q.most), pages, w, lane, [&](int key, f32x4 d) {
-        if (key < key1)
-          for (int k = 0; k < 4; ++k) {
-            const int r = (4 * o + k) % kR;
-            if (r0 + r < p.R) base[size_t(r) * stride + key] = d[k];
-          }
+  const size_t stride = size_t(p.span) * p.nsplit, gs = stride / kGranule, row0 = size_t(bh) * p.R + r0;
+  float* base = p.scores + row0 * stride;
+  float* gbase = p.gmax + row0 * gs;
+  score_keys<kScoreWaves>(
+      p, q, h, key0, min(key1, q.most), pages, w, lane,
+      [&](int key, f32x4 d) {
+        for (int k = 0; k < 4; ++k) {
+          const int r = (4 * o + k) % kR;
+          if (key < key1 && r0 + r < p.R) base[size_t(r) * stride + key] = d[k];
+        }
+      },
+      [&](int granule, int r, float m) {
+        if (r0 + r < p.R) gbase[size_t(r) * gs + granule] = m;
       });
 }
 
 // Split plan, second launch: one block per row.
 template <typename T, int NG, int NW>
 __global__ __launch_bounds__(NW * kWave) void cache_row_kernel(CacheAttnParams p) {
-  constexpr int kCap = 1024 / NW;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[team_lds_bytes<NW, kCap>()];
+  __shared__ TeamLds<NW, NW == 16 ? 256 : 512> L;
+  __shared__ float lz[kList];
+  __shared__ int li[kList];
   const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   const int row = blockIdx.x % p.R, bh = blockIdx.x / p.R;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
-  const float* sp = p.scores + (size_t(bh) * p.R + row) * (size_t(p.span) * p.nsplit);
-  finish_row<T, NG, NW, kCap>(p, b, h, row, visible_keys(p, b, row % p.NQ), sp, team_lds<NW, kCap>(smem), w, 0, NW,
-                              lane);
+  const size_t at = size_t(bh) * p.R + row, stride = size_t(p.span) * p.nsplit;
+  finish_row<T, NG, NW, true>(p, b, h, row, visible_keys(p, b, row % p.NQ), p.gmax + at * (stride / kGranule),
+                              p.scores + at * stride, L, lz, li, w, 0, NW, lane);
 }
 
 template <typename K> hipError_t allow_lds(K kern, size_t lds) {
@@ -690,8 +761,10 @@ int tiles_shared(const CacheAttnParams& p, int dtype) {
 
 size_t one_lds_bytes(const CacheAttnParams& p, int tile_rows, int* stride) {
   const int rows = p.R < tile_rows ? p.R : tile_rows;
-  *stride = (p.maxlen + 63) / 64 * 64 + 4;
-  return team_lds_bytes<kOneWaves, kOneCap>() + size_t(rows) * *stride * 4 +
+  *stride = (p.maxlen + kGranule - 1) / kGranule * kGranule;
+  int pad = 1;
+  while (pad < rows && pad < kOneWaves) pad *= 2;
+  return size_t(rows) * (*stride + *stride / kGranule) * 4 + size_t(pad) * kList * 8 +
          size_t((p.maxlen + p.c.page - 1) / p.c.page + 1) * 4;
 }
 
@@ -749,7 +822,8 @@ size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus) {
   const int tile_rows = kTile / tiles_shared(p, dtype);
   int stride = 0;
   p.span = p.nsplit = 0;
-  if (p.maxlen <= 2048 && one_lds_bytes(p, tile_rows, &stride) <= max_lds) {
+  if (p.maxlen <= 2048 &&
+      one_lds_bytes(p, tile_rows, &stride) + sizeof(OneLds) <= max_lds) {
     p.plan = kCacheOneBlock;
     return 0;
   }
@@ -762,10 +836,15 @@ size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus) {
   if (span > 4096) span = 4096;
   p.span = int(span);
   p.nsplit = int((p.maxlen + span - 1) / span);
-  return size_t(p.B) * p.c.heads * p.R * p.nsplit * size_t(p.span) * sizeof(float);
+  return size_t(p.B) * p.c.heads * p.R * p.nsplit * (size_t(p.span) + p.span / kGranule) * sizeof(float);
 }
 
-hipError_t launch_cache_attn(const CacheAttnParams& p, int dtype, hipStream_t s) {
+hipError_t launch_cache_attn(const CacheAttnParams& call, int dtype, hipStream_t s) {
+  CacheAttnParams p = call;
+  p.e = 1.0f / (p.alpha - 1.0f);
+  p.pc = pow_class_of(p.e);
+  p.zc = (p.alpha - 1.0f) * (p.scale < 0.0f ? -p.scale : p.scale);
+  p.zb = 10.0f * (p.alpha - 1.0f);
   if (dtype == kElemBF16) return launch_t<u16>(p, dtype, s);
   if (dtype == kElemF16) return launch_t<h16>(p, dtype, s);
   return launch_t<float>(p, dtype, s);
