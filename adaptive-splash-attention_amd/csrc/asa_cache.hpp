@@ -85,13 +85,19 @@ struct CacheAttnParams {
   int pc;                 // pow_class_of(e)
   int plan;               // CachePlan
   int span, nsplit;       // split plan: keys per score block, score blocks per row tile
-  float* scores;          // split plan: dots, [B * c.heads * R, span * nsplit]
-  float* gmax;            // split plan: each 64 keys' maxima, [B * c.heads * R, span * nsplit / 64]
+  int tile_rows;          // split plan: query rows that share a score block
+  // split plan, rows = min(tile_rows, R), tiles of them per key head, n =
+  // span * nsplit: dots [B * c.heads, tiles, n / 64, rows, 64], and each 64
+  // keys' maxima [B * c.heads, tiles, rows, n / 64]
+  float* scores;
+  float* gmax;
 };
 // How attention runs: one block per 16 rows that holds their scores in LDS,
 // or the keys split over score blocks, then one block per row.
 enum CachePlan : int { kCacheOneBlock = 0, kCacheSplit = 1 };
-// Fills plan, span and nsplit; returns the workspace bytes.
+// Rows of the workspace's tensors (B * c.heads * tiles * rows).
+size_t cache_score_rows(const CacheAttnParams& p);
+// Fills plan, span, nsplit and tile_rows; returns the workspace bytes.
 size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus);
 hipError_t launch_cache_attn(const CacheAttnParams& p, int dtype, hipStream_t s);
 

@@ -60,138 +60,205 @@ template <typename T> using CodeVec = typename Half<CodeType<T>>::v8;
 // 8 codes as 16 + c: channels 0 4 1 5 2 6 3 7, since nibbles j and j + 4 are
 // 16 bits apart.  The query operand has the same order.
 __device__ __forceinline__ int operand_slot(int j) { return j < 4 ? 2 * j : 2 * j - 7; }
-template <typename T> __device__ __forceinline__ CodeVec<T> codes_operand(uint32_t w) {
-  uint32_t u[4];
-  if constexpr (std::is_same<T, h16>::value) {  // 16.0 = 0x4c00, one = 1 << 6
-    const uint32_t mask = 0x03c003c0u, one = 0x4c004c00u;
-    u[0] = ((w << 6) & mask) | one;
-    u[1] = ((w << 2) & mask) | one;
-    u[2] = ((w >> 2) & mask) | one;
-    u[3] = ((w >> 6) & mask) | one;
-  } else {  // 16.0 = 0x4180, one = 1 << 3
-    const uint32_t mask = 0x00780078u, one = 0x41804180u;
-    u[0] = ((w << 3) & mask) | one;
-    u[1] = ((w >> 1) & mask) | one;
-    u[2] = ((w >> 5) & mask) | one;
-    u[3] = ((w >> 9) & mask) | one;
-  }
-  CodeVec<T> r;
-  __builtin_memcpy(&r, u, 16);
-  return r;
-}
-
-// One wave's query operand: rows r0 .. of a key head's R rows (row r: query
-// head h * rep + r / NQ, token r % NQ), kR of them, for each of the P key
-// tiles that share a result, and the accumulators' starts.  Queries of a
-// negative scale are negated, so that larger products are larger scores.
-template <typename T, int P, int NG>
-struct QueryFrag {
-  static constexpr int kR = kTile / P;
-  static constexpr int NT = std::is_same<T, float>::value ? 3 : 1;
-  CodeVec<T> a[P][NG][NT];
-  f32x4 bias[NG];  // -16 sum q_g of rows (4 (lane / 16) + k) % kR
-  int vis[4];      // visible keys of those rows
-  int most, least; // over the real rows of the tile
-
-  __device__ __forceinline__ void load(const CacheAttnParams& p, int b, int h, int r0, int lane) {
-    using S = typename Half<CodeType<T>>::scalar;
-    const int o = lane >> 4, ar = lane & 15, r = r0 + ar % kR;
-    const bool ok = r < p.R;
-    const int rr = ok ? r : 0, head = h * p.rep + rr / p.NQ, i = rr % p.NQ;
-    const T* q = static_cast<const T*>(p.q) + size_t(b) * p.lq.sb + size_t(head) * p.lq.sh + size_t(i) * p.lq.sn;
-    const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int ch = 32 * g + 8 * o, nv = ok ? p.c.hd - ch : 0;
-      float x[8];
-      if (p.chunks) {
-        constexpr int kEpc = 16 / int(sizeof(T));
-        T e[8] = {};
-        if (nv > 0)
-          for (int c = 0; c < 8; c += kEpc) {
-            const uint4 u = *reinterpret_cast<const uint4*>(q + ch + c);
-            __builtin_memcpy(e + c, &u, 16);
-          }
-        for (int j = 0; j < 8; ++j) x[j] = Elem<T>::load(e + j);
-      } else {
-        for (int j = 0; j < 8; ++j) x[j] = j < nv ? Elem<T>::load(q + ch + j) : 0.0f;
-      }
-      for (int j = 0; j < 8; ++j) x[j] *= sign;
-      const float sum = sum_groups(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
-      for (int k = 0; k < 4; ++k) bias[g][k] = -16.0f * __shfl(sum, 4 * o + k, 64);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        for (int j = 0; j < 8; ++j) {
-          const S y = static_cast<S>(x[j]);
-          x[j] -= static_cast<float>(y);
-          for (int u = 0; u < P; ++u) a[u][g][t][operand_slot(j)] = ar / kR == u ? y : static_cast<S>(0.0f);
-        }
+// mask and one are held in registers (v_and_or_b32 takes no literals).
+template <typename T> struct Codes {
+  static constexpr bool kF16 = std::is_same<T, h16>::value;
+  uint32_t mask = kF16 ? 0x03c003c0u : 0x00780078u;
+  uint32_t one = kF16 ? 0x4c004c00u : 0x41804180u;  // 16.0; the codes' unit is 1 << 6, 1 << 3
+  __device__ __forceinline__ Codes() { asm("" : "+s"(mask), "+v"(one)); }
+  __device__ __forceinline__ CodeVec<T> operator()(uint32_t w) const {
+    uint32_t u[4];
+    if constexpr (kF16) {
+      u[0] = ((w << 6) & mask) | one;
+      u[1] = ((w << 2) & mask) | one;
+      u[2] = ((w >> 2) & mask) | one;
+      u[3] = ((w >> 6) & mask) | one;
+    } else {
+      u[0] = ((w << 3) & mask) | one;
+      u[1] = ((w >> 1) & mask) | one;
+      u[2] = ((w >> 5) & mask) | one;
+      u[3] = ((w >> 9) & mask) | one;
     }
-    int hi = 0, lo = INT_MAX;
-    for (int k = 0; k < 4; ++k) {
-      const int row = r0 + (4 * o + k) % kR;
-      vis[k] = row < p.R ? visible_keys(p, b, row % p.NQ) : 0;
-      hi = max(hi, vis[k]);
-      lo = row < p.R ? min(lo, vis[k]) : lo;
-    }
-    most = wave_reduce_minmax<true>(hi);
-    least = wave_reduce_minmax<false>(lo);
+    CodeVec<T> r;
+    __builtin_memcpy(&r, u, 16);
+    return r;
   }
 };
 
-// P tiles of 16 keys: the codes (key order: lane group o has octet o of every
-// channel group) of key lane % 16 of each tile, and the params of the lane's
-// own key of the result.
+// The query operand of a tile of rows r0 .. of a key head's R rows (row r:
+// query head h * rep + r / NQ, token r % NQ), kR of them, in LDS: a lane of
+// tile u reads its row's 8 channels if its operand row is one of tile u's,
+// and the zeros behind each group's entries if not.  In registers the P
+// operands would take 64 of them and the occupancy that hides the loads.
+template <typename T, int P, int NG>
+struct QueryLds {
+  static constexpr int kR = kTile / P;
+  static constexpr int NT = std::is_same<T, float>::value ? 3 : 1;
+  uint4 a[NG][NT][4 * kR + 1];  // [..][octet * kR + row], zeros
+  alignas(16) float bias[NG][kTile];  // -16 sum q_g of each row
+};
+
+// 8 channels of a query row from `ch` on, zeros past the head dimension.
+template <typename T>
+__device__ __forceinline__ void load_query(const CacheAttnParams& p, const T* q, int ch, float* x) {
+  const int nv = p.c.hd - ch;
+  if (p.chunks) {
+    constexpr int kEpc = 16 / int(sizeof(T));
+    T e[8] = {};
+    if (nv > 0)
+      for (int c = 0; c < 8; c += kEpc) {
+        const uint4 u = *reinterpret_cast<const uint4*>(q + ch + c);
+        __builtin_memcpy(e + c, &u, 16);
+      }
+    for (int j = 0; j < 8; ++j) x[j] = Elem<T>::load(e + j);
+  } else {
+    for (int j = 0; j < 8; ++j) x[j] = j < nv ? Elem<T>::load(q + ch + j) : 0.0f;
+  }
+}
+
+// Fills ql by the block's `waves` waves, a channel group each; queries of a
+// negative scale are negated, so that larger products are larger scores.
+template <typename T, int P, int NG>
+__device__ __forceinline__ void stage_query(const CacheAttnParams& p, QueryLds<T, P, NG>& ql, int b, int h, int r0,
+                                            int w, int waves, int lane) {
+  using S = typename Half<CodeType<T>>::scalar;
+  using QL = QueryLds<T, P, NG>;
+  constexpr int kR = QL::kR;
+  const int o = lane >> 4, r = lane & 15;
+  const bool ok = r < kR && r0 + r < p.R;
+  const int rr = ok ? r0 + r : 0, head = h * p.rep + rr / p.NQ, i = rr % p.NQ;
+  const T* q = static_cast<const T*>(p.q) + size_t(b) * p.lq.sb + size_t(head) * p.lq.sh + size_t(i) * p.lq.sn;
+  const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+  for (int g = w; g < NG; g += waves) {
+    float x[8];
+    load_query<T>(p, q, 32 * g + 8 * o, x);
+    for (int j = 0; j < 8; ++j) x[j] = ok ? x[j] * sign : 0.0f;
+    const float sum = sum_groups(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
+    if (o == 0) ql.bias[g][r] = -16.0f * sum;
+#pragma unroll
+    for (int t = 0; t < QL::NT; ++t) {
+      CodeVec<T> v;
+      for (int j = 0; j < 8; ++j) {
+        const S y = static_cast<S>(x[j]);
+        x[j] -= static_cast<float>(y);
+        v[operand_slot(j)] = y;
+      }
+      uint4 u;
+      __builtin_memcpy(&u, &v, 16);
+      if (r < kR) ql.a[g][t][o * kR + r] = u;
+      if (lane == 0) ql.a[g][t][4 * kR] = uint4{0u, 0u, 0u, 0u};
+    }
+  }
+}
+
+// Where a wave reads the operand, and what its rows see.
+template <int P>
+struct TileRows {
+  static constexpr int kR = kTile / P;
+  int at[P];       // entry of QueryLds::a for tile u
+  int bias;        // and of its bias, for the result's rows
+  int vis[4];      // visible keys of rows (4 (lane / 16) + k) % kR
+  int most, least; // over the real rows of the tile
+  // row whose granule maximum the lane has after granule_maxima
+  __device__ __forceinline__ static int max_row(int lane) {
+    const int o = lane >> 4;
+    return P == 4 ? o : P == 2 ? 4 * (o & 1) + (o & 2) + (lane & 1) : 4 * o + (lane & 3);
+  }
+  __device__ __forceinline__ void load(const CacheAttnParams& p, int b, int r0, int lane) {
+    const int o = lane >> 4, ar = lane & 15, row = r0 + ar % kR;
+    for (int u = 0; u < P; ++u) at[u] = ar / kR == u ? o * kR + ar % kR : 4 * kR;
+    bias = (4 * o) % kR;
+    const int v = row < p.R ? visible_keys(p, b, row % p.NQ) : 0;
+    most = wave_reduce_minmax<true>(v);
+    least = wave_reduce_minmax<false>(row < p.R ? v : INT_MAX);
+    for (int k = 0; k < 4; ++k) vis[k] = __shfl(v, (4 * o + k) % kR, 64);
+  }
+};
+
+// A granule: 64 keys, four tiles of 16 in 4 / P packs of P tiles that share a
+// result.  The codes (key order: lane group o has octet o of every channel
+// group) of key lane % 16 of each tile, and the params of the lane's own key
+// of each pack's result.
+constexpr int kGranule = 64;
 template <int P, int NG>
-struct KeyPack {
-  uint32_t w[P][NG], pr[NG];
-  bool seen;  // the lane's own key has a page
+struct KeyGranule {
+  static constexpr int V = 4 / P;
+  uint32_t w[4][NG], pr[V][NG];
+  bool seen[V];  // the lane's own key has a page
+  bool whole;    // every key of the granule has one (wave-uniform)
 
   template <int N> static __device__ __forceinline__ void words(uint32_t* d, const uint32_t* s) {
     __builtin_memcpy(d, __builtin_assume_aligned(s, N == 4 ? 16 : N == 2 ? 8 : 4), 4 * N);
   }
-  // keys base .. base + 16 P - 1 of [.., key1); pages: of the keys from key0
+  // keys base .. base + 63 of [.., key1); pages: of the keys from key0
   __device__ __forceinline__ void load(const CachePool& c, int h, const int* pages, int key0, int base, int key1,
                                        int lane) {
     const int o = lane >> 4, col = lane & 15;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(c.k_codes);
+    if (c.page >= kGranule) {  // one page: its address is the wave's, the rest a constant of the lane
+      const int pg = __builtin_amdgcn_readfirstlane(pages[(base - key0) >> c.page_shift]);
+      const bool on = pg >= 0;
+      const size_t row = (size_t(on ? pg : 0) * c.heads + h) * c.page + (base & (c.page - 1));
+      const uint32_t* cw = codes + row * (4 * NG);
+      const uint32_t* cp = c.k_params + row * NG;
 #pragma unroll
-    for (int u = 0; u < P; ++u) {
-      const int key = base + kTile * u;
-      const int pg = key < key1 ? __builtin_amdgcn_readfirstlane(pages[(key - key0) >> c.page_shift]) : -1;
-      if (pg >= 0) {
-        const int64_t row = (int64_t(pg) * c.heads + h) * c.page + (key & (c.page - 1)) + col;
-        words<NG>(w[u], reinterpret_cast<const uint32_t*>(c.k_codes) + row * (4 * NG) + NG * o);
-      } else {
-        for (int g = 0; g < NG; ++g) w[u][g] = 0u;
+      for (int u = 0; u < 4; ++u) words<NG>(w[u], cw + (kTile * u + col) * (4 * NG) + NG * o);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        seen[v] = on;
+        words<NG>(pr[v], cp + (kTile * (P * v + o * P / 4) + col) * NG);
+      }
+      whole = on;
+    } else {
+      whole = true;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = base + kTile * u;
+        const int pg = key < key1 ? __builtin_amdgcn_readfirstlane(pages[(key - key0) >> c.page_shift]) : -1;
+        whole = whole && pg >= 0;
+        const size_t row = (size_t(pg >= 0 ? pg : 0) * c.heads + h) * c.page + (key & (c.page - 1));
+        words<NG>(w[u], codes + row * (4 * NG) + col * (4 * NG) + NG * o);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int key = base + kTile * (P * v + o * P / 4);
+        const int pg = key < key1 ? pages[(key - key0) >> c.page_shift] : -1;
+        seen[v] = pg >= 0;
+        const size_t row = (size_t(pg >= 0 ? pg : 0) * c.heads + h) * c.page + (key & (c.page - 1)) + col;
+        words<NG>(pr[v], c.k_params + row * NG);
       }
     }
-    const int key = base + kTile * (o * P / 4);
-    const int pg = key < key1 ? pages[(key - key0) >> c.page_shift] : -1;
-    seen = pg >= 0;
-    for (int g = 0; g < NG; ++g) pr[g] = 0u;
-    if (seen) words<NG>(pr, c.k_params + ((int64_t(pg) * c.heads + h) * c.page + (key & (c.page - 1)) + col) * NG);
   }
 };
 
-// q.k: element k of a lane is row (4 (lane / 16) + k) % kR, key
-// 16 (lane / 16 * P / 4) + lane % 16 of the pack.
+// q.k: element k of s[v] is row (4 (lane / 16) + k) % kR, key
+// 16 (P v + lane / 16 * P / 4) + lane % 16 of the granule.
 template <typename T, int P, int NG>
-__device__ __forceinline__ f32x4 dots(const QueryFrag<T, P, NG>& q, const KeyPack<P, NG>& k) {
-  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+__device__ __forceinline__ void dots(const QueryLds<T, P, NG>& ql, const TileRows<P>& t, const KeyGranule<P, NG>& k,
+                                     const Codes<T>& codes, f32x4* s) {
+  constexpr int V = 4 / P, NT = QueryLds<T, P, NG>::NT;
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    f32x4 acc = q.bias[g];
+    const f32x4 bias = *reinterpret_cast<const f32x4*>(&ql.bias[g][t.bias]);
+    CodeVec<T> a[P][NT];
 #pragma unroll
-    for (int u = 0; u < P; ++u) {
-      const CodeVec<T> c = codes_operand<T>(k.w[u][g]);
+    for (int u = 0; u < P; ++u)
+      for (int i = 0; i < NT; ++i) __builtin_memcpy(&a[u][i], &ql.a[g][i][t.at[u]], 16);
 #pragma unroll
-      for (int t = 0; t < QueryFrag<T, P, NG>::NT; ++t) acc = mfma(q.a[u][g][t], c, acc);
+    for (int v = 0; v < V; ++v) {
+      f32x4 acc = bias;
+#pragma unroll
+      for (int u = 0; u < P; ++u) {
+        const CodeVec<T> c = codes(k.w[P * v + u][g]);
+        for (int i = 0; i < NT; ++i) acc = mfma(a[u][i], c, acc);
+      }
+      const float sc = __uint_as_float(k.pr[v][g] << 16);
+      const float off = __uint_as_float(k.pr[v][g] & 0xffff0000u) * -0.0625f;  // m sum q_g = -m / 16 bias
+      for (int r = 0; r < 4; ++r) s[v][r] = fmaf(off, bias[r], fmaf(sc, acc[r], s[v][r]));
     }
-    const float sc = __uint_as_float(k.pr[g] << 16);
-    const float off = __uint_as_float(k.pr[g] & 0xffff0000u) * -0.0625f;  // m sum q_g = -m / 16 bias
-    for (int r = 0; r < 4; ++r) s[r] = fmaf(off, q.bias[g][r], fmaf(sc, acc[r], s[r]));
   }
-  return s;
 }
 
 // z = (alpha - 1) clamp(|scale| dot), hidden keys apart.
@@ -214,63 +281,118 @@ __device__ __forceinline__ void stage_pages(const CacheAttnParams& p, int b, int
   }
 }
 
-// Dots of the keys [key0, key1) by the block's NW waves, a granule of 64 keys
-// per wave and step (4 / P packs; the next step's loads are in flight
-// meanwhile), handed to put(key, dots) (dots as from `dots`; hidden where a
-// row does not see the key); the granule's maxima of each row to
-// most(granule, row of the tile, maximum) by one lane.  key0 is a multiple of
-// the page size and of 64.
-constexpr int kGranule = 64;
-template <int NW, typename T, int P, int NG, typename Put, typename Most>
-__device__ __forceinline__ void score_keys(const CacheAttnParams& p, const QueryFrag<T, P, NG>& q, int h,
-                                           int key0, int key1, const int* pages, int w, int lane,
-                                           Put put, Most most) {
-  constexpr int V = 4 / P, kKeys = kTile * P, kR = kTile / P;
-  const int own = kTile * ((lane >> 4) * P / 4) + (lane & 15);
-  KeyPack<P, NG> next[V];
-  int base = key0 + w * kGranule;
-  if (base < key1)
-#pragma unroll
-    for (int v = 0; v < V; ++v) next[v].load(p.c, h, pages, key0, base + v * kKeys, key1, lane);
-  for (; base < key1; base += NW * kGranule) {
-    KeyPack<P, NG> k[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) k[v] = next[v];
-    const int ahead = base + NW * kGranule;
-    if (ahead < key1)
-#pragma unroll
-      for (int v = 0; v < V; ++v) next[v].load(p.c, h, pages, key0, ahead + v * kKeys, key1, lane);
-    f32x4 m = {kHidden, kHidden, kHidden, kHidden};
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int first = base + v * kKeys, key = first + own;
-      if (first < key1) {
-        f32x4 d = dots<T, P, NG>(q, k[v]);
-        for (int r = 0; r < 4; ++r) d[r] = fmaxf(d[r], kNotNumber);
-        if (first + kKeys > q.least)
-          for (int r = 0; r < 4; ++r) d[r] = key < q.vis[r] ? d[r] : kHidden;
-        for (int r = 0; r < 4; ++r) d[r] = k[v].seen ? d[r] : kHidden;
-        put(key, d);
-        for (int r = 0; r < 4; ++r) m[r] = fmaxf(m[r], d[r]);
-      }
+// The granule's maximum of the row TileRows::max_row(lane), from the maxima m
+// over the lane's own keys: halves and rows are exchanged first, so that
+// later steps work on one register, then lanes of a 16-lane row that share
+// the query row are reduced by rotations.
+template <int R> __device__ __forceinline__ float max_ror(float x) {  // with the lane R further in its 16
+  return fmaxf(x, __uint_as_float(dpp_mov<0x120 + R>(__float_as_uint(x))));
+}
+__device__ __forceinline__ float max_swap32(float x, float y) {  // lanes 0-31: x, 32-63: y, over both halves
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float max_swap16(float x, float y) {  // even 16-lane rows: x, odd: y, over pairs
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+template <int P> __device__ __forceinline__ float granule_maxima(const f32x4& m, int lane) {
+  if constexpr (P == 4) {
+    float x = max_swap16(max_swap32(m[0], m[2]), max_swap32(m[1], m[3]));
+    x = max_ror<1>(x);
+    x = max_ror<2>(x);
+    x = max_ror<4>(x);
+    return max_ror<8>(x);
+  } else {
+    // lanes with bit k of their number set take y, the others x, over pairs
+    auto merge1 = [lane](float x, float y) {
+      const bool odd = lane & 1;
+      return fmaxf(odd ? y : x, __uint_as_float(lane_xor<1>(__float_as_uint(odd ? x : y))));
+    };
+    if constexpr (P == 2) {
+      float x = merge1(max_swap32(m[0], m[2]), max_swap32(m[1], m[3]));
+      x = max_ror<2>(x);
+      x = max_ror<4>(x);
+      return max_ror<8>(x);
+    } else {
+      const float x = merge1(m[0], m[1]), y = merge1(m[2], m[3]);
+      const bool two = lane & 2;
+      float z = fmaxf(two ? y : x, __uint_as_float(lane_xor<2>(__float_as_uint(two ? x : y))));
+      z = max_ror<4>(z);
+      return max_ror<8>(z);
     }
+  }
+}
+
+// Dots of the keys [key0, key1) by the block's NW waves, a granule per wave
+// and step (the next step's loads are in flight meanwhile), into
+// out[(granule * rows + row) * 64 + key % 64], granule = key / 64, and each
+// granule's maxima into gmax[row * gstride + granule].  Rows whose largest z
+// in a granule is not above that of the wave's granules so far less one can
+// have no weight there: their dots are left out.  key0 is a multiple of the
+// page size and of 64.
+template <int NW, typename T, int P, int NG>
+__device__ __forceinline__ void score_keys(const CacheAttnParams& p, const QueryLds<T, P, NG>& ql,
+                                           const TileRows<P>& tr, int h, int key0, int key1, const int* pages,
+                                           int rows, float* out, float* gmax, size_t gstride, int w, int lane) {
+  constexpr int V = 4 / P, kR = kTile / P;
+  const int o = lane >> 4, own = kTile * (o * P / 4) + (lane & 15), mrow = tr.max_row(lane);
+  const ZOf zof(p);
+  const Codes<T> codes;
+  // lanes that store their row's maximum
+  const bool teller = mrow < rows && (lane & 15) == (P == 4 ? 0 : P == 2 ? (lane & 1) : (lane & 3));
+  float* gm = gmax + size_t(mrow < rows ? mrow : 0) * gstride;
+  float bound = kHidden;
+  auto step = [&](int base, const KeyGranule<P, NG>& k) {
+    // the operand is read again for every granule (empty, not volatile asm:
+    // the reads stay in the loop, and nothing else is ordered by it)
+    TileRows<P> t = tr;
+    for (int u = 0; u < P; ++u) asm("" : "+v"(t.at[u]) : "s"(base));
+    asm("" : "+v"(t.bias) : "s"(base));
+    f32x4 d[V];
+    dots<T, P, NG>(ql, t, k, codes, d);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      for (int r = 0; r < 4; ++r) d[v][r] = fmaxf(d[v][r], kNotNumber);
+    if (!k.whole || base + kGranule > t.least)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        for (int r = 0; r < 4; ++r)
+          d[v][r] = k.seen[v] && base + kTile * P * v + own < t.vis[r] ? d[v][r] : kHidden;
+    f32x4 m = d[0];
+    for (int v = 1; v < V; ++v)
+      for (int r = 0; r < 4; ++r) m[r] = fmaxf(m[r], d[v][r]);
+    const float x = granule_maxima<P>(m, lane);
+    if (teller) gm[base / kGranule] = x;
+    const float z = zof(x);
+    const uint64_t want = __ballot(z > bound && mrow < rows);
+    bound = fmaxf(bound, z - 1.0f);
+    float* og = out + size_t(base / kGranule) * (rows * kGranule);
+#pragma unroll
     for (int r = 0; r < 4; ++r) {
-      float x = m[r];
-      x = fmaxf(x, __uint_as_float(lane_xor<1>(__float_as_uint(x))));
-      x = fmaxf(x, __uint_as_float(lane_xor<2>(__float_as_uint(x))));
-      x = fmaxf(x, __uint_as_float(lane_xor<7>(__float_as_uint(x))));
-      x = fmaxf(x, __uint_as_float(lane_xor<15>(__float_as_uint(x))));
-      if constexpr (P >= 2) {
-        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-      }
+      // bits of the lanes that have row (4 o + r) % kR
       if constexpr (P == 4) {
-        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+        if ((want >> (16 * r)) & 1) og[r * kGranule + own] = d[0][r];
+      } else {
+        const int row = (4 * o + r) % kR;
+        const int bit = P == 2 ? 16 * (o & 1) + 32 * (r >> 1) + (r & 1) : 16 * o + r;
+        if ((want >> bit) & 1)
+          for (int v = 0; v < V; ++v) og[row * kGranule + kTile * P * v + own] = d[v][r];
       }
-      const int row = 4 * (lane >> 4) + r;
-      if ((lane & 15) == 0 && row < kR) most(base / kGranule, row, x);
     }
+  };
+  constexpr int kStep = NW * kGranule;
+  KeyGranule<P, NG> ka, kb;
+  int base = key0 + w * kGranule;
+  if (base < key1) ka.load(p.c, h, pages, key0, base, key1, lane);
+  while (base < key1) {
+    if (base + kStep < key1) kb.load(p.c, h, pages, key0, base + kStep, key1, lane);
+    step(base, ka);
+    base += kStep;
+    if (base >= key1) break;
+    if (base + kStep < key1) ka.load(p.c, h, pages, key0, base + kStep, key1, lane);
+    step(base, kb);
+    base += kStep;
   }
 }
 
@@ -396,15 +518,16 @@ struct ValueSum {
   }
 };
 
-// tau and the output of row `row` (of the key head's R) from its dots at
-// sp[0 .. vis) and their granule maxima gp, by `size` waves of the block from
+// tau and the output of row `row` (of the key head's R) from its dots (key j at
+// sp[j / 64 * gstep + j % 64], where its granule may hold a weight) and its
+// granule maxima gp, by `size` waves of the block from
 // wave w0 on; lz, li: kList entries of (z, key) of the team.  Every wave of
 // the block calls it together (teams meet at the block's barriers); row = -1,
 // vis = 0 for a team without a row.  WHOLE: the team is the block.
 template <typename T, int NG, int NW, bool WHOLE, typename Lds>
 __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int h, int row, int vis,
-                                           const float* gp, const float* sp, Lds& L, float* lz, int* li, int w,
-                                           int w0, int size, int lane) {
+                                           const float* gp, const float* sp, int gstep, Lds& L, float* lz, int* li,
+                                           int w, int w0, int size, int lane) {
   constexpr int kCap = Lds::kCap;
   const int member = w - w0, pc = p.pc;
   const float e = p.e;
@@ -474,8 +597,9 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
           for (int k = 0; k < 4; ++k) {
             const int l = todo ? __builtin_ctzll(todo) : -1;
             todo &= todo - 1;
-            key[k] = l < 0 ? vis : (i0 + l * size + member) * kGranule + lane;
-            d[k] = sp[key[k] < vis ? key[k] : 0];
+            const int gi = l < 0 ? 0 : i0 + l * size + member;
+            key[k] = l < 0 ? vis : gi * kGranule + lane;
+            d[k] = sp[size_t(gi) * gstep + lane];
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) collect(d[k], key[k]);
@@ -507,9 +631,11 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
     float F = 0.0f, F1 = 0.0f;
     if (!listed && !dense) {
 #pragma unroll 4
-      for (int j = member * kWave + lane; j < vis; j += size * kWave) {
+      for (int i = member; i < ng; i += size) {
+        const int j = i * kGranule + lane;
+        const bool in = j < vis && zof(gp[i]) > lo;  // the others hold no dots
         float pa, pa1;
-        powers(pc, fmaxf(zof(sp[j]) - tau, 0.0f), e, pa, pa1);
+        powers(pc, fmaxf(in ? zof(sp[size_t(i) * gstep + lane]) - tau : 0.0f, 0.0f), e, pa, pa1);
         F += pa;
         F1 += pa1;
       }
@@ -601,7 +727,9 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
         float zj = kHidden;
         int key = 0;
         if (j < cnt) {
-          zj = small ? lz[k0 + j] : big ? L.cz[w][j] : zof(sp[k0 + j]);
+          const int gi = (k0 + j) / kGranule;
+          zj = small ? lz[k0 + j] : big ? L.cz[w][j]
+               : zof(gp[gi]) > lo ? zof(sp[size_t(gi) * gstep + (k0 + j) % kGranule]) : kHidden;
           key = small ? li[k0 + j] : big ? L.ci[w][j] : k0 + j;
         }
         float pa, pa1;
@@ -655,11 +783,11 @@ __global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnP
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ OneLds L;
   constexpr int kR = kTile / P;
-  const int t = threadIdx.x, w = t >> 6, lane = t & 63, o = lane >> 4;
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   const int nrt = (p.R + kR - 1) / kR;
-  const int rt = blockIdx.x % nrt, bh = blockIdx.x / nrt;
+  const int tile = blockIdx.x % nrt, bh = blockIdx.x / nrt;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
-  const int r0 = rt * kR, rows = min(kR, p.R - r0), most = min(kR, p.R), gs = stride / kGranule;
+  const int r0 = tile * kR, rows = min(kR, p.R - r0), most = min(kR, p.R), gs = stride / kGranule;
   int pad = 1;
   while (pad < most && pad < kOneWaves) pad *= 2;
   float* zs = reinterpret_cast<float*>(smem);
@@ -668,22 +796,13 @@ __global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnP
   int* li = reinterpret_cast<int*>(lz + pad * kList);
   int* pages = li + pad * kList;
   stage_pages(p, b, 0, p.maxlen, pages, t, kOneWaves * kWave);
-  const int len = max(0, min(p.lengths[b], p.maxlen));
+  __shared__ QueryLds<T, P, NG> ql;
+  stage_query<T, P, NG>(p, ql, b, h, r0, w, kOneWaves, lane);
   {
-    QueryFrag<T, P, NG> q;
-    q.load(p, b, h, r0, lane);
+    TileRows<P> rt;
+    rt.load(p, b, r0, lane);
     __syncthreads();
-    score_keys<kOneWaves>(
-        p, q, h, 0, min(len, q.most), pages, w, lane,
-        [&](int key, f32x4 d) {
-          for (int k = 0; k < 4; ++k) {
-            const int r = (4 * o + k) % kR;
-            if (r < rows) zs[r * stride + key] = d[k];
-          }
-        },
-        [&](int granule, int r, float m) {
-          if (r < rows) gs0[r * gs + granule] = m;
-        });
+    score_keys<kOneWaves>(p, ql, rt, h, 0, rt.most, pages, most, zs, gs0, gs, w, lane);
   }
   __syncthreads();
   const int size = kOneWaves / pad, team = w / size, w0 = team * size;
@@ -691,46 +810,36 @@ __global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnP
     const int r = first + team;
     const bool has = r < rows;
     finish_row<T, NG, kOneWaves, false>(p, b, h, has ? r0 + r : -1, has ? visible_keys(p, b, (r0 + r) % p.NQ) : 0,
-                                        gs0 + (has ? r : 0) * gs, zs + (has ? r : 0) * stride, L, lz + team * kList,
-                                        li + team * kList, w, w0, size, lane);
+                                        gs0 + (has ? r : 0) * gs, zs + (has ? r : 0) * kGranule, most * kGranule, L,
+                                        lz + team * kList, li + team * kList, w, w0, size, lane);
   }
 }
 
 // Split plan, first launch: dots of `span` keys with a tile of rows, and
 // their granules' maxima.
 template <typename T, int P, int NG>
-__global__ __launch_bounds__(kScoreWaves * kWave) void cache_score_kernel(CacheAttnParams p) {
+__global__ __launch_bounds__(kScoreWaves * kWave, 4) void cache_score_kernel(CacheAttnParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int kR = kTile / P;
   int* pages = reinterpret_cast<int*>(smem);
-  const int t = threadIdx.x, w = t >> 6, lane = t & 63, o = lane >> 4;
+  __shared__ QueryLds<T, P, NG> ql;
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   const int nrt = (p.R + kR - 1) / kR;
   const int split = blockIdx.x % p.nsplit, rest = blockIdx.x / p.nsplit;
-  const int rt = rest % nrt, bh = rest / nrt;
+  const int tile = rest % nrt, bh = rest / nrt;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
-  const int r0 = rt * kR;
+  const int r0 = tile * kR;
   const int key0 = split * p.span;
-  const int len = max(0, min(p.lengths[b], p.maxlen));
-  if (key0 >= len) return;
-  const int key1 = min(len, key0 + p.span);
-  stage_pages(p, b, key0, key1 - key0, pages, t, kScoreWaves * kWave);
-  QueryFrag<T, P, NG> q;
-  q.load(p, b, h, r0, lane);
+  stage_pages(p, b, key0, min(p.span, p.maxlen - key0), pages, t, kScoreWaves * kWave);
+  stage_query<T, P, NG>(p, ql, b, h, r0, w, kScoreWaves, lane);
+  TileRows<P> rt;
+  rt.load(p, b, r0, lane);
+  if (key0 >= rt.most) return;  // block-uniform
   __syncthreads();
-  const size_t stride = size_t(p.span) * p.nsplit, gs = stride / kGranule, row0 = size_t(bh) * p.R + r0;
-  float* base = p.scores + row0 * stride;
-  float* gbase = p.gmax + row0 * gs;
-  score_keys<kScoreWaves>(
-      p, q, h, key0, min(key1, q.most), pages, w, lane,
-      [&](int key, f32x4 d) {
-        for (int k = 0; k < 4; ++k) {
-          const int r = (4 * o + k) % kR;
-          if (key < key1 && r0 + r < p.R) base[size_t(r) * stride + key] = d[k];
-        }
-      },
-      [&](int granule, int r, float m) {
-        if (r0 + r < p.R) gbase[size_t(r) * gs + granule] = m;
-      });
+  const int rows = min(kR, p.R);
+  const size_t gs = size_t(p.span / kGranule) * p.nsplit, row0 = (size_t(bh) * nrt + tile) * rows;
+  score_keys<kScoreWaves>(p, ql, rt, h, key0, min(key0 + p.span, rt.most), pages, rows,
+                          p.scores + row0 * gs * kGranule, p.gmax + row0 * gs, gs, w, lane);
 }
 
 // Split plan, second launch: one block per row.
@@ -742,9 +851,12 @@ __global__ __launch_bounds__(NW * kWave) void cache_row_kernel(CacheAttnParams p
   const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   const int row = blockIdx.x % p.R, bh = blockIdx.x / p.R;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
-  const size_t at = size_t(bh) * p.R + row, stride = size_t(p.span) * p.nsplit;
-  finish_row<T, NG, NW, true>(p, b, h, row, visible_keys(p, b, row % p.NQ), p.gmax + at * (stride / kGranule),
-                              p.scores + at * stride, L, lz, li, w, 0, NW, lane);
+  // the score blocks' tiles of `rows` rows
+  const int rows = min(p.tile_rows, p.R), nrt = (p.R + rows - 1) / rows, tile = row / rows, r = row % rows;
+  const size_t gs = size_t(p.span / kGranule) * p.nsplit, row0 = (size_t(bh) * nrt + tile) * rows;
+  finish_row<T, NG, NW, true>(p, b, h, row, visible_keys(p, b, row % p.NQ), p.gmax + (row0 + r) * gs,
+                              p.scores + row0 * gs * kGranule + r * kGranule, rows * kGranule, L, lz, li, w, 0, NW,
+                              lane);
 }
 
 template <typename K> hipError_t allow_lds(K kern, size_t lds) {
@@ -753,10 +865,10 @@ template <typename K> hipError_t allow_lds(K kern, size_t lds) {
                              int(lds));
 }
 
-// Key tiles that share a result: as many as leave room for the rows.  fp32
-// queries (three terms) would need P times their 48 operand registers.
+// Key tiles that share a result: as many as leave room for the rows, two at
+// most for fp32 queries (three operand reads of LDS for each).
 int tiles_shared(const CacheAttnParams& p, int dtype) {
-  return dtype == kElemF32 || p.R > 8 ? 1 : p.R > 4 ? 2 : 4;
+  return p.R > 8 ? 1 : p.R > 4 || dtype == kElemF32 ? 2 : 4;
 }
 
 size_t one_lds_bytes(const CacheAttnParams& p, int tile_rows, int* stride) {
@@ -792,7 +904,7 @@ template <typename T, int NG>
 hipError_t launch_ng(const CacheAttnParams& p, int dtype, hipStream_t s) {
   hipError_t e = hipSuccess;
   if constexpr (std::is_same<T, float>::value) {
-    e = launch_png<T, 1, NG>(p, s);
+    e = p.R > 8 ? launch_png<T, 1, NG>(p, s) : launch_png<T, 2, NG>(p, s);
   } else {
     const int P = tiles_shared(p, dtype);
     e = P == 1 ? launch_png<T, 1, NG>(p, s) : P == 2 ? launch_png<T, 2, NG>(p, s) : launch_png<T, 4, NG>(p, s);
@@ -818,12 +930,18 @@ hipError_t launch_t(const CacheAttnParams& p, int dtype, hipStream_t s) {
 
 }  // namespace
 
+size_t cache_score_rows(const CacheAttnParams& p) {
+  const int rows = p.R < p.tile_rows ? p.R : p.tile_rows;
+  return size_t(p.B) * p.c.heads * ((p.R + rows - 1) / rows) * rows;
+}
+
 size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus) {
   const int tile_rows = kTile / tiles_shared(p, dtype);
+  p.tile_rows = tile_rows;
   int stride = 0;
   p.span = p.nsplit = 0;
   if (p.maxlen <= 2048 &&
-      one_lds_bytes(p, tile_rows, &stride) + sizeof(OneLds) <= max_lds) {
+      one_lds_bytes(p, tile_rows, &stride) + sizeof(OneLds) + 16384 <= max_lds) {
     p.plan = kCacheOneBlock;
     return 0;
   }
@@ -836,7 +954,7 @@ size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus) {
   if (span > 4096) span = 4096;
   p.span = int(span);
   p.nsplit = int((p.maxlen + span - 1) / span);
-  return size_t(p.B) * p.c.heads * p.R * p.nsplit * (size_t(p.span) + p.span / kGranule) * sizeof(float);
+  return cache_score_rows(p) * p.nsplit * (size_t(p.span) + p.span / kGranule) * sizeof(float);
 }
 
 hipError_t launch_cache_attn(const CacheAttnParams& call, int dtype, hipStream_t s) {

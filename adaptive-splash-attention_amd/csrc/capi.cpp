@@ -907,7 +907,7 @@ int asa_cache_attention(const asa_cache* c, const asa_cache_query* a, const void
   ap.chunks = whole_chunks(q, ap.lq, c->head_dim, a->dtype);
   ap.out = out;
   ap.scores = static_cast<float*>(workspace);
-  ap.gmax = ap.scores + size_t(ap.B) * ap.c.heads * ap.R * ap.span * ap.nsplit;
+  ap.gmax = ap.scores + asa::cache_score_rows(ap) * ap.span * ap.nsplit;
   if (int rc = check_hip(asa::launch_cache_attn(ap, a->dtype, static_cast<hipStream_t>(stream)),
                          "cache attention kernel launch"))
     return rc;
