@@ -412,6 +412,20 @@ template <typename F> __device__ __forceinline__ float wave_reduce(float v, F op
 __device__ __forceinline__ float wave_sum(float v) {
   return wave_reduce(v, [](float a, float b) { return a + b; });
 }
+// The sums of x and of y over the wave: lanes 0-31 go on with x, the others
+// with y, so that both take the steps of one.
+__device__ __forceinline__ void wave_sum2(float& x, float& y) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  float v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  v += __uint_as_float(lane_xor<1>(__float_as_uint(v)));
+  v += __uint_as_float(lane_xor<2>(__float_as_uint(v)));
+  v += __uint_as_float(lane_xor<7>(__float_as_uint(v)));
+  v += __uint_as_float(lane_xor<15>(__float_as_uint(v)));
+  const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(t[0]) + __uint_as_float(t[1]);
+  x = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 0));
+  y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 32));
+}
 __device__ __forceinline__ float wave_max(float v) {
   return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
@@ -443,7 +457,7 @@ __device__ __forceinline__ bool next_tau(float alpha, float F, float F1, float& 
   else hi = tau;
   float nt = 0.5f * (lo + hi);
   if (alpha <= 2.0f) {
-    const float s = tau + (F - __builtin_amdgcn_exp2f((2.0f - alpha) * __builtin_amdgcn_logf(F))) / F1;
+    const float s = tau + (F - __builtin_amdgcn_exp2f((2.0f - alpha) * __builtin_amdgcn_logf(F))) * __builtin_amdgcn_rcpf(F1);
     if (s >= lo && s <= hi) nt = s;
   }
   const bool done = nt == tau || nt == lo || fabsf(f) <= (alpha <= 2.0f ? 1e-6f : 1e-7f);
@@ -452,9 +466,7 @@ __device__ __forceinline__ bool next_tau(float alpha, float F, float F1, float& 
 }
 constexpr int kMaxSteps = 64;
 
-// LDS of the row teams.  A wave collects up to CAP candidates of its row; a
-// list of up to kList is gathered for the whole team (8 registers of a wave).
-constexpr int kList = 512;
+// LDS of the row teams.  A wave collects up to CAP candidates of its row.
 constexpr int kAccStride = 132;
 template <int NW, int CAP> struct TeamLds {
   static constexpr int kCap = CAP;
@@ -462,49 +474,57 @@ template <int NW, int CAP> struct TeamLds {
   int ci[NW][CAP];
   float gm[NW][kWave];
   float red[2][NW][2];
+  float say[NW][4];   // from a team's first wave: zmax, lo; tau, the sum at tau
   float psum[NW];
   int cnt[NW];
   float acc[NW][kAccStride];
 };
 
 // Adds p_j v_j of the wave's listed keys to the lane's 8 channels: CL lanes
-// have a row's octets, so a step takes 64 / CL entries, four loads deep.
+// have a row's octets, so four loads in flight take 4 * 64 / CL entries.
 template <int NG>
 struct ValueSum {
-  static constexpr int kCl = NG == 3 ? 16 : 4 * NG, kPer = kWave / kCl;
+  static constexpr int kCl = NG == 3 ? 16 : 4 * NG, kPer = kWave / kCl, kStep = 4 * kPer;
   float acc[8] = {};
   float off = 0.0f;
-  __device__ __forceinline__ void add(const CacheAttnParams& p, int b, int h, const float* pz, const int* pi,
-                                      int n, int lane) {
+  uint32_t w[4], pr[4];
+  __device__ __forceinline__ void load(const CacheAttnParams& p, int b, int h, const int* pi, int e0, int n, int lane) {
     const int c = lane & (kCl - 1), slot = lane / kCl, g = c >> 2;
     const int32_t* table = p.table + size_t(b) * p.cols;
-    for (int e0 = 0; e0 < n; e0 += 4 * kPer) {
-      uint32_t w[4], pr[4];
-      float pj[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int e = e0 + u * kPer + slot;
-        w[u] = pr[u] = 0u;
-        pj[u] = 0.0f;
-        if (e < n && g < NG) {
-          const int64_t row = cache_row(p.c, table, p.cols, pi[e], h);
-          if (row >= 0) {
-            pj[u] = pz[e];
-            w[u] = reinterpret_cast<const uint32_t*>(p.c.v_codes)[row * (4 * NG) + c];
-            pr[u] = p.c.v_params[row * NG + g];
-          }
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * kPer + slot;
+      w[u] = pr[u] = 0u;
+      if (e < n && g < NG) {
+        const int64_t row = cache_row(p.c, table, p.cols, pi[e], h);
+        if (row >= 0) {
+          w[u] = reinterpret_cast<const uint32_t*>(p.c.v_codes)[row * (4 * NG) + c];
+          pr[u] = p.c.v_params[row * NG + g];
         }
       }
+    }
+  }
+  // weights pz[e] of the entries that load was given
+  __device__ __forceinline__ void use(const float* pz, int e0, int n, int lane) {
+    const int slot = lane / kCl;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float ps = pj[u] * __uint_as_float(pr[u] << 16);
-        off = fmaf(pj[u], __uint_as_float(pr[u] & 0xffff0000u), off);
-        const uint32_t even = w[u] & 0x0f0f0f0fu, odd = (w[u] >> 4) & 0x0f0f0f0fu;
-        for (int j = 0; j < 4; ++j) {
-          acc[2 * j] = fmaf(ps, float((even >> (8 * j)) & 255u), acc[2 * j]);
-          acc[2 * j + 1] = fmaf(ps, float((odd >> (8 * j)) & 255u), acc[2 * j + 1]);
-        }
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * kPer + slot;
+      const float pj = e < n ? pz[e] : 0.0f;
+      const float ps = pj * __uint_as_float(pr[u] << 16);
+      off = fmaf(pj, __uint_as_float(pr[u] & 0xffff0000u), off);
+      const uint32_t even = w[u] & 0x0f0f0f0fu, odd = (w[u] >> 4) & 0x0f0f0f0fu;
+      for (int j = 0; j < 4; ++j) {
+        acc[2 * j] = fmaf(ps, float((even >> (8 * j)) & 255u), acc[2 * j]);
+        acc[2 * j + 1] = fmaf(ps, float((odd >> (8 * j)) & 255u), acc[2 * j + 1]);
       }
+    }
+  }
+  __device__ __forceinline__ void add(const CacheAttnParams& p, int b, int h, const float* pz, const int* pi, int n,
+                                      int lane) {
+    for (int e0 = 0; e0 < n; e0 += kStep) {
+      load(p, b, h, pi, e0, n, lane);
+      use(pz, e0, n, lane);
     }
   }
   // the wave's sums of channels 8 c + j, in every lane with that c
@@ -520,59 +540,70 @@ struct ValueSum {
 
 // tau and the output of row `row` (of the key head's R) from its dots (key j at
 // sp[j / 64 * gstep + j % 64], where its granule may hold a weight) and its
-// granule maxima gp, by `size` waves of the block from
-// wave w0 on; lz, li: kList entries of (z, key) of the team.  Every wave of
-// the block calls it together (teams meet at the block's barriers); row = -1,
-// vis = 0 for a team without a row.  WHOLE: the team is the block.
+// granule maxima gp, by `size` waves of the block from wave w0 on.  Every
+// wave of the block calls it together (teams meet at the block's barriers);
+// row = -1, vis = 0 for a team without a row.  WHOLE: the team is the block.
+// The Newton steps are a team's first wave's: the same steps on every wave
+// would share the SIMDs with one another.  Meanwhile the others load the
+// values of their candidates.
 template <typename T, int NG, int NW, bool WHOLE, typename Lds>
 __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int h, int row, int vis,
-                                           const float* gp, const float* sp, int gstep, Lds& L, float* lz, int* li,
-                                           int w, int w0, int size, int lane) {
+                                           const float* gp, const float* sp, int gstep, Lds& L, int w, int w0,
+                                           int size, int lane) {
   constexpr int kCap = Lds::kCap;
   const int member = w - w0, pc = p.pc;
   const float e = p.e;
   const ZOf zof(p);
 
   // ---- the largest z, and a bound below tau from the granules' ----
+  // granule i is member i % size's
   const int ng = (vis + kGranule - 1) / kGranule;
-  float g = kHidden;
-#pragma unroll 4
-  for (int j = member * kWave + lane; j < ng; j += size * kWave) g = fmaxf(g, gp[j]);
-  L.gm[w][lane] = zof(g);
+  const int g0 = lane * size + member;
+  const float gfirst = g0 < ng ? zof(gp[g0]) : kHidden;
+  float g = gfirst;
+  for (int i = g0 + size * kWave; i < ng; i += size * kWave) g = fmaxf(g, zof(gp[i]));
+  L.gm[w][lane] = g;
   __syncthreads();
-  float gz[4] = {kHidden, kHidden, kHidden, kHidden};
-  for (int i = 0; i < size; i += 4)
+  if (member == 0) {
+    float gz[4] = {kHidden, kHidden, kHidden, kHidden};
+    for (int i = 0; i < size; i += 4)
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (i + k < size) gz[k] = fmaxf(gz[k], L.gm[w0 + i + k][lane]);
-  const float zmax = wave_max(fmaxf(fmaxf(gz[0], gz[1]), fmaxf(gz[2], gz[3])));
-  const bool empty = !(zmax > 0.5f * kHidden);
-  float tau = zmax - 1.0f, lo = tau, hi = zmax;
-  if (vis > kList && !empty) {
-    // a few steps: any tau left of the root of the maxima will do
-    for (int it = 0; it < 12; ++it) {
-      float F = 0.0f, F1 = 0.0f;
+      for (int k = 0; k < 4; ++k)
+        if (i + k < size) gz[k] = fmaxf(gz[k], L.gm[w + i + k][lane]);
+    const float zm = wave_max(fmaxf(fmaxf(gz[0], gz[1]), fmaxf(gz[2], gz[3])));
+    float t = zm - 1.0f, lo = t, hi = zm;
+    if (ng > 1 && zm > 0.5f * kHidden) {
+      // a few steps: any tau left of the root of the maxima will do, and near
+      // the root a step drops few candidates
+      for (int it = 0; it < 12; ++it) {
+        float F = 0.0f, F1 = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float pa, pa1;
-        powers(pc, fmaxf(gz[k] - tau, 0.0f), e, pa, pa1);
-        F += pa;
-        F1 += pa1;
+        for (int k = 0; k < 4; ++k) {
+          float pa, pa1;
+          powers(pc, fmaxf(gz[k] - t, 0.0f), e, pa, pa1);
+          F += pa;
+          F1 += pa1;
+        }
+        wave_sum2(F, F1);
+        if (F < 1.5f && p.alpha <= 2.0f) break;
+        if (next_tau(p.alpha, F, F1, t, lo, hi)) break;
       }
-      F = wave_sum(F);
-      if (F < 1.01f && p.alpha <= 2.0f) break;
-      if (next_tau(p.alpha, F, wave_sum(F1), tau, lo, hi)) break;
+      // less the rounding of the steps, and of F at them
+      lo = fmaxf((p.alpha <= 2.0f ? t : lo) - 4e-6f, zm - 1.0f);
     }
-    // the rounding of the steps, and of F at them
-    if (p.alpha <= 2.0f) lo = tau;
-    lo = fmaxf(lo - 4e-6f, zmax - 1.0f);
-    tau = lo;
-    hi = zmax;
+    if (lane == 0) {
+      L.say[w][0] = zm;
+      L.say[w][1] = lo;
+    }
   }
+  __syncthreads();
+  const float zmax = L.say[w0][0];
+  const bool empty = !(zmax > 0.5f * kHidden);
+  float lo = L.say[w0][1], tau = lo, hi = zmax;
 
   // ---- the keys with z > lo, listed; lo moves up while they do not fit ----
-  bool listed = false, big = false, dense = empty;
-  int n = 0, mine = 0;
+  bool listed = false, dense = empty;
+  int most = 0, mine = 0;  // the longest of the team's lists
   for (int it = 0;; ++it) {
     if (!listed && !dense) {
       mine = 0;
@@ -586,45 +617,34 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
         }
         mine += __builtin_popcountll(m);
       };
-      // granule i is member i % size's
       for (int i0 = 0; i0 < ng; i0 += size * kWave) {
-        const int i = i0 + lane * size + member;
-        uint64_t todo = __ballot(i < ng && zof(gp[i < ng ? i : 0]) > lo);
+        const int i = i0 + g0;
+        uint64_t todo = __ballot(i < ng && (i0 ? zof(gp[i < ng ? i : 0]) : gfirst) > lo);
         while (todo) {
-          float d[4];
-          int key[4];
+          constexpr int kDeep = 8;  // granules in flight
+          float d[kDeep];
+          int key[kDeep];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < kDeep; ++k) {
             const int l = todo ? __builtin_ctzll(todo) : -1;
             todo &= todo - 1;
             const int gi = l < 0 ? 0 : i0 + l * size + member;
             key[k] = l < 0 ? vis : gi * kGranule + lane;
-            d[k] = sp[size_t(gi) * gstep + lane];
+            d[k] = kHidden;
+            if (l >= 0) d[k] = sp[size_t(gi) * gstep + lane];
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) collect(d[k], key[k]);
+          for (int k = 0; k < kDeep; ++k)
+            collect(d[k], key[k]);
         }
       }
       if (lane == 0) L.cnt[w] = mine;
     }
     __syncthreads();
     if (!listed && !dense) {
-      n = 0;
-      int before = 0;
-      bool fits = true;
-      for (int i = 0; i < size; ++i) {
-        const int c = L.cnt[w0 + i];
-        if (i == member) before = n;
-        n += c;
-        fits = fits && c <= kCap;
-      }
-      listed = fits && (WHOLE || n <= kList);
-      big = listed && n > kList;
-      if (listed && !big)
-        for (int j = lane; j < mine; j += kWave) {
-          lz[before + j] = L.cz[w][j];
-          li[before + j] = L.ci[w][j];
-        }
+      most = 0;
+      for (int i = 0; i < size; ++i) most = max(most, L.cnt[w0 + i]);
+      listed = most <= kCap;
     }
     if (!__syncthreads_or(!listed && !dense)) break;
     // some team's candidates did not fit: one step of its tau over the whole row
@@ -639,8 +659,7 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
         F += pa;
         F1 += pa1;
       }
-      F = wave_sum(F);
-      F1 = wave_sum(F1);
+      wave_sum2(F, F1);
       if (lane == 0) {
         L.red[0][w][0] = F;
         L.red[0][w][1] = F1;
@@ -658,68 +677,102 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
     }
   }
 
-  // ---- tau over the list ----
+  // ---- tau over the lists ----
+  ValueSum<NG> vs;
+  const bool few = listed && mine <= ValueSum<NG>::kStep;
+  if (few) vs.load(p, b, h, L.ci[w], 0, mine, lane);
   float total = 0.0f;
-  if (listed) {
+  if (WHOLE && listed && most > kWave) {  // each wave its own
     tau = lo;
     bool done = false;
-    if (!big) {  // in registers, by every wave alike
-      constexpr int kRegs = kList / kWave;
-      float z[kRegs];
-#pragma unroll
-      for (int k = 0; k < kRegs; ++k) z[k] = k * kWave + lane < n ? lz[k * kWave + lane] : kHidden;
-      for (int it = 0; it <= kMaxSteps; ++it) {
-        float F = 0.0f, F1 = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kRegs; ++k)
-          if (k * kWave < n) {
-            float pa, pa1;
-            powers(pc, fmaxf(z[k] - tau, 0.0f), e, pa, pa1);
-            F += pa;
-            F1 += pa1;
-          }
-        total = wave_sum(F);
-        if (done || it == kMaxSteps) break;  // the sum at the final tau
-        done = next_tau(p.alpha, total, wave_sum(F1), tau, lo, hi);
-      }
-    } else {  // each wave its candidates; the block's barriers are the team's
-      for (int it = 0; it <= kMaxSteps; ++it) {
-        float F = 0.0f, F1 = 0.0f;
+    for (int it = 0; it <= kMaxSteps; ++it) {
+      float F = 0.0f, F1 = 0.0f;
 #pragma unroll 2
-        for (int j = lane; j < mine; j += kWave) {
-          float pa, pa1;
-          powers(pc, fmaxf(L.cz[w][j] - tau, 0.0f), e, pa, pa1);
-          F += pa;
-          F1 += pa1;
-        }
-        F = wave_sum(F);
-        F1 = wave_sum(F1);
-        if (lane == 0) {
-          L.red[it & 1][w][0] = F;
-          L.red[it & 1][w][1] = F1;
-        }
-        __syncthreads();
-        total = F1 = 0.0f;
-        for (int i = 0; i < size; ++i) {
-          total += L.red[it & 1][i][0];
-          F1 += L.red[it & 1][i][1];
-        }
-        if (done || it == kMaxSteps) break;
-        done = next_tau(p.alpha, total, F1, tau, lo, hi);
+      for (int j = lane; j < mine; j += kWave) {
+        float pa, pa1;
+        powers(pc, fmaxf(L.cz[w][j] - tau, 0.0f), e, pa, pa1);
+        F += pa;
+        F1 += pa1;
       }
+      wave_sum2(F, F1);
+      if (lane == 0) {
+        L.red[it & 1][w][0] = F;
+        L.red[it & 1][w][1] = F1;
+      }
+      __syncthreads();
+      total = F1 = 0.0f;
+      for (int i = 0; i < NW; ++i) {
+        total += L.red[it & 1][i][0];
+        F1 += L.red[it & 1][i][1];
+      }
+      if (done || it == kMaxSteps) break;  // the sum at the final tau
+      done = next_tau(p.alpha, total, F1, tau, lo, hi);
+    }
+    __syncthreads();
+  } else {
+    if (listed && member == 0) {
+      float t = lo;
+      bool done = false;
+      auto steps = [&](auto sums) {
+        for (int it = 0; it <= kMaxSteps; ++it) {
+          float F = 0.0f, F1 = 0.0f;
+          sums(t, F, F1);
+          wave_sum2(F, F1);
+          total = F;
+          if (done || it == kMaxSteps) break;
+          done = next_tau(p.alpha, total, F1, t, lo, hi);
+        }
+      };
+      if (most <= kWave) {  // a register for each wave's list
+        float z[NW];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) z[i] = i < size && lane < L.cnt[w + i] ? L.cz[w + i][lane] : kHidden;
+        steps([&](float at, float& F, float& F1) {
+#pragma unroll
+          for (int i = 0; i < NW; ++i)
+            if (i < size) {
+              float pa, pa1;
+              powers(pc, fmaxf(z[i] - at, 0.0f), e, pa, pa1);
+              F += pa;
+              F1 += pa1;
+            }
+        });
+      } else {
+        steps([&](float at, float& F, float& F1) {
+          for (int i = 0; i < size; ++i)
+            for (int j = lane; j < L.cnt[w + i]; j += kWave) {
+              float pa, pa1;
+              powers(pc, fmaxf(L.cz[w + i][j] - at, 0.0f), e, pa, pa1);
+              F += pa;
+              F1 += pa1;
+            }
+        });
+      }
+      if (lane == 0) {
+        L.say[w][2] = t;
+        L.say[w][3] = total;
+      }
+    }
+    __syncthreads();
+    if (listed) {
+      tau = L.say[w0][2];
+      total = L.say[w0][3];
     }
   }
 
   // ---- the support's weights and values ----
-  ValueSum<NG> vs;
   float psum = 0.0f;
-  if (!empty) {
-    // the wave's part of the list, or its candidates, or its keys of the
-    // row, kCap at a time
-    const bool small = listed && !big;
-    const int part = small ? (n + size - 1) / size : big ? mine : kCap;
-    const int end = small ? min(n, (member + 1) * part) : big ? mine : vis;
-    for (int k0 = big ? 0 : member * part; k0 < end; k0 += size * part) {
+  if (few) {
+    for (int j = lane; j < mine; j += kWave) {
+      float pa, pa1;
+      powers(pc, fmaxf(L.cz[w][j] - tau, 0.0f), e, pa, pa1);
+      L.cz[w][j] = pa;
+    }
+    vs.use(L.cz[w], 0, mine, lane);
+  } else if (!empty) {
+    // the wave's candidates, or its keys of the row, kCap at a time
+    const int part = listed ? mine : kCap, end = listed ? mine : vis;
+    for (int k0 = listed ? 0 : member * part; k0 < end; k0 += size * part) {
       const int cnt = min(part, end - k0);
       int c = 0;
       for (int j0 = 0; j0 < cnt; j0 += kWave) {
@@ -728,9 +781,8 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
         int key = 0;
         if (j < cnt) {
           const int gi = (k0 + j) / kGranule;
-          zj = small ? lz[k0 + j] : big ? L.cz[w][j]
-               : zof(gp[gi]) > lo ? zof(sp[size_t(gi) * gstep + (k0 + j) % kGranule]) : kHidden;
-          key = small ? li[k0 + j] : big ? L.ci[w][j] : k0 + j;
+          zj = listed ? L.cz[w][j] : zof(gp[gi]) > lo ? zof(sp[size_t(gi) * gstep + (k0 + j) % kGranule]) : kHidden;
+          key = listed ? L.ci[w][j] : k0 + j;
         }
         float pa, pa1;
         powers(pc, fmaxf(zj - tau, 0.0f), e, pa, pa1);
@@ -774,7 +826,7 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
 
 constexpr int kOneWaves = 8;    // one-block plan
 constexpr int kScoreWaves = 4;  // split plan: score blocks
-constexpr int kRowKeys = 8192;  // split plan: rows up to this have 4 waves, else 16
+constexpr int kRowKeys = 8192;  // split plan: rows up to this have 4 waves, else 8
 
 // One block per tile of rows of a key head: dots into LDS, then its rows.
 using OneLds = TeamLds<kOneWaves, 128>;
@@ -792,9 +844,7 @@ __global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnP
   while (pad < most && pad < kOneWaves) pad *= 2;
   float* zs = reinterpret_cast<float*>(smem);
   float* gs0 = zs + most * stride;  // granule maxima
-  float* lz = gs0 + most * gs;      // a list for each of `pad` teams
-  int* li = reinterpret_cast<int*>(lz + pad * kList);
-  int* pages = li + pad * kList;
+  int* pages = reinterpret_cast<int*>(gs0 + most * gs);
   stage_pages(p, b, 0, p.maxlen, pages, t, kOneWaves * kWave);
   __shared__ QueryLds<T, P, NG> ql;
   stage_query<T, P, NG>(p, ql, b, h, r0, w, kOneWaves, lane);
@@ -810,8 +860,8 @@ __global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnP
     const int r = first + team;
     const bool has = r < rows;
     finish_row<T, NG, kOneWaves, false>(p, b, h, has ? r0 + r : -1, has ? visible_keys(p, b, (r0 + r) % p.NQ) : 0,
-                                        gs0 + (has ? r : 0) * gs, zs + (has ? r : 0) * kGranule, most * kGranule, L,
-                                        lz + team * kList, li + team * kList, w, w0, size, lane);
+                                        gs0 + (has ? r : 0) * gs, zs + (has ? r : 0) * kGranule, most * kGranule, L, w,
+                                        w0, size, lane);
   }
 }
 
@@ -845,9 +895,7 @@ __global__ __launch_bounds__(kScoreWaves * kWave, 4) void cache_score_kernel(Cac
 // Split plan, second launch: one block per row.
 template <typename T, int NG, int NW>
 __global__ __launch_bounds__(NW * kWave) void cache_row_kernel(CacheAttnParams p) {
-  __shared__ TeamLds<NW, NW == 16 ? 256 : 512> L;
-  __shared__ float lz[kList];
-  __shared__ int li[kList];
+  __shared__ TeamLds<NW, 512> L;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   const int row = blockIdx.x % p.R, bh = blockIdx.x / p.R;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
@@ -855,8 +903,7 @@ __global__ __launch_bounds__(NW * kWave) void cache_row_kernel(CacheAttnParams p
   const int rows = min(p.tile_rows, p.R), nrt = (p.R + rows - 1) / rows, tile = row / rows, r = row % rows;
   const size_t gs = size_t(p.span / kGranule) * p.nsplit, row0 = (size_t(bh) * nrt + tile) * rows;
   finish_row<T, NG, NW, true>(p, b, h, row, visible_keys(p, b, row % p.NQ), p.gmax + (row0 + r) * gs,
-                              p.scores + row0 * gs * kGranule + r * kGranule, rows * kGranule, L, lz, li, w, 0, NW,
-                              lane);
+                              p.scores + row0 * gs * kGranule + r * kGranule, rows * kGranule, L, w, 0, NW, lane);
 }
 
 template <typename K> hipError_t allow_lds(K kern, size_t lds) {
@@ -874,9 +921,7 @@ int tiles_shared(const CacheAttnParams& p, int dtype) {
 size_t one_lds_bytes(const CacheAttnParams& p, int tile_rows, int* stride) {
   const int rows = p.R < tile_rows ? p.R : tile_rows;
   *stride = (p.maxlen + kGranule - 1) / kGranule * kGranule;
-  int pad = 1;
-  while (pad < rows && pad < kOneWaves) pad *= 2;
-  return size_t(rows) * (*stride + *stride / kGranule) * 4 + size_t(pad) * kList * 8 +
+  return size_t(rows) * (*stride + *stride / kGranule) * 4 +
          size_t((p.maxlen + p.c.page - 1) / p.c.page + 1) * 4;
 }
 
@@ -913,7 +958,7 @@ hipError_t launch_ng(const CacheAttnParams& p, int dtype, hipStream_t s) {
   const dim3 grid(unsigned(p.B) * p.c.heads * p.R);
   profile_begin("cache_row", s);
   if (p.maxlen <= kRowKeys) hipLaunchKernelGGL((cache_row_kernel<T, NG, 4>), grid, dim3(4 * kWave), 0, s, p);
-  else hipLaunchKernelGGL((cache_row_kernel<T, NG, 16>), grid, dim3(16 * kWave), 0, s, p);
+  else hipLaunchKernelGGL((cache_row_kernel<T, NG, 8>), grid, dim3(8 * kWave), 0, s, p);
   profile_end(s);
   return hipGetLastError();
 }
