@@ -95,10 +95,25 @@ struct CacheAttnParams {
 // How attention runs: one block per 16 rows that holds their scores in LDS,
 // or the keys split over score blocks, then one block per row.
 enum CachePlan : int { kCacheOneBlock = 0, kCacheSplit = 1 };
+// Keys whose maxima are kept together, and the static LDS of a one-block
+// kernel beside its dots (an upper bound).
+constexpr int kCacheGranule = 64;
+constexpr size_t kCacheOneStatic = 32768;
+// One-block plan: dynamic LDS bytes, and the keys of a row there.
+inline size_t cache_one_lds(const CacheAttnParams& p, int* stride) {
+  const int rows = p.R < p.tile_rows ? p.R : p.tile_rows;
+  *stride = (p.maxlen + kCacheGranule - 1) / kCacheGranule * kCacheGranule;
+  return size_t(rows) * (*stride + *stride / kCacheGranule) * 4 +
+         size_t((p.maxlen + p.c.page - 1) / p.c.page + 1) * 4;
+}
 // Rows of the workspace's tensors (B * c.heads * tiles * rows).
 size_t cache_score_rows(const CacheAttnParams& p);
 // Fills plan, span, nsplit and tile_rows; returns the workspace bytes.
 size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus);
 hipError_t launch_cache_attn(const CacheAttnParams& p, int dtype, hipStream_t s);
+// By the queries' type (one translation unit each).
+hipError_t launch_cache_attn_bf16(const CacheAttnParams& p, hipStream_t s);
+hipError_t launch_cache_attn_f16(const CacheAttnParams& p, hipStream_t s);
+hipError_t launch_cache_attn_f32(const CacheAttnParams& p, hipStream_t s);
 
 }  // namespace asa

@@ -1,0 +1,8 @@
+// Attention over the 4-bit cache (cache_attn_kernel.hpp) for bf16 queries.
+#include "cache_attn_kernel.hpp"
+
+namespace asa {
+
+hipError_t launch_cache_attn_bf16(const CacheAttnParams& p, hipStream_t s) { return launch_cache_attn_t<u16>(p, s); }
+
+}  // namespace asa

@@ -322,8 +322,9 @@ int validate_cache(const asa_cache* c, bool pointers, asa::CachePool* pool) {
     return fail(ASA_ERR_INVALID_ARGUMENT, "Head dimension too large (%d > 128)", c->head_dim);
   if (c->head_dim < 1)
     return fail(ASA_ERR_INVALID_ARGUMENT, "head_dim %d must be >= 1", c->head_dim);
-  if ((long long)c->pages * c->kv_heads > (1LL << 40) / c->page_size)
-    return fail(ASA_ERR_INVALID_ARGUMENT, "cache too large");
+  if ((long long)c->pages * c->page_size >= (1LL << 31))
+    return fail(ASA_ERR_INVALID_ARGUMENT, "cache too large: pages (%d) x page_size (%d) tokens must be below 2^31",
+                c->pages, c->page_size);
   if (pointers) {
     if (!c->k_codes || !c->v_codes || !c->k_params || !c->v_params)
       return fail(ASA_ERR_INVALID_ARGUMENT, "a cache tensor is NULL");

@@ -20,9 +20,9 @@ BUILD = os.path.join(ROOT, "_build")
 LIBDIR = os.path.join(PKG_DIR, "lib")
 LIB = os.path.join(LIBDIR, "libadasplash.so")
 
-SOURCES = ["sparse_bwd.hip", "cache_attn.hip", "select_bf16.hip", "select_f16.hip", "select_f32.hip", "forward.hip",
+SOURCES = ["sparse_bwd.hip", "cache_attn_f32.hip", "cache_attn_bf16.hip", "cache_attn_f16.hip", "select_bf16.hip", "select_f16.hip", "select_f32.hip", "forward.hip",
            "backward.hip", "exact.hip", "select.hip", "compact.hip", "check.hip",
-           "cache.hip", "capi.cpp"]
+           "cache.hip", "cache_attn.hip", "capi.cpp"]
 ARCH = "gfx950"
 FLAGS = [
     f"--offload-arch={ARCH}",

@@ -288,7 +288,7 @@ int asa_check_nonfinite(int32_t dtype, int32_t count, const void* const* tensors
  * position past max_pages, or whose entry is not a page of the pool, has no
  * row: it is not written, reads as zeros, and no query sees it.           */
 typedef struct asa_cache {
-  int32_t pages;     /* >= 1                                               */
+  int32_t pages;     /* >= 1; pages * page_size below 2^31                 */
   int32_t kv_heads;
   int32_t page_size; /* tokens of a page: 16, 32, 64, 128 or 256           */
   int32_t head_dim;  /* 1..128                                             */

@@ -128,7 +128,7 @@ def _c(**kw):
 
 
 @pytest.mark.parametrize("bad,msg", [
-    (dict(pages=0), "pages"), (dict(kv_heads=0), "kv_heads"), (dict(page_size=24), "page_size"),
+    (dict(pages=0), "pages"), (dict(pages=1 << 27), "too large"), (dict(kv_heads=0), "kv_heads"), (dict(page_size=24), "page_size"),
     (dict(page_size=512), "page_size"), (dict(head_dim=129), "too large"), (dict(head_dim=0), "head_dim"),
     (dict(k_codes=None), "NULL"), (dict(v_params=(1 << 20) + 8), "aligned"),
 ])
