@@ -427,12 +427,18 @@ int validate_query(const asa_cache* c, const asa_cache_query* a, bool pointers,
 
 // Chooses how the call runs on the current device; its workspace bytes.
 int plan_query(asa::CacheAttnParams* ap, int dtype, size_t* bytes) {
-  int dev = 0, max_lds = 0, cus = 0;
+  // LDS of a block by device ordinal: asked once (a serving step makes many calls)
+  static std::atomic<int> cached[64] = {};
+  int dev = 0, cus = 0;
   if (int rc = check_hip(hipGetDevice(&dev), "hipGetDevice")) return rc;
-  if (int rc = check_hip(hipDeviceGetAttribute(&max_lds, hipDeviceAttributeMaxSharedMemoryPerBlock,
-                                               dev),
-                         "hipDeviceGetAttribute"))
-    return rc;
+  int max_lds = dev >= 0 && dev < 64 ? cached[dev].load() : 0;
+  if (max_lds == 0) {
+    if (int rc = check_hip(hipDeviceGetAttribute(&max_lds,
+                                                 hipDeviceAttributeMaxSharedMemoryPerBlock, dev),
+                           "hipDeviceGetAttribute"))
+      return rc;
+    if (dev >= 0 && dev < 64) cached[dev].store(max_lds);
+  }
   if (int rc = device_cus(&cus)) return rc;
   *bytes = asa::cache_attn_plan(*ap, dtype, size_t(max_lds), cus);
   const long long blocks = (long long)ap->B * ap->c.heads * ((ap->R + 15) / 16) *

@@ -28,6 +28,9 @@ GROUP = 32           # channels that share a scale and an offset
 def _i32(t, shape, device, name: str) -> torch.Tensor:
     """An integer argument as contiguous int32 on `device`; values outside
     int32 become its bounds (no page, or a length past every page)."""
+    if (type(t) is torch.Tensor and t.dtype is torch.int32 and t.shape == shape
+            and t.device == device and t.is_contiguous()):
+        return t  # the common case: one comparison each
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
@@ -44,16 +47,30 @@ def _i32(t, shape, device, name: str) -> torch.Tensor:
     return t.contiguous()
 
 
+def _table(t, rows, device) -> torch.Tensor:
+    """A page table [rows, P] (rows None: any)."""
+    if (type(t) is torch.Tensor and t.dtype is torch.int32 and t.dim() == 2 and t.device == device
+            and (rows is None or t.size(0) == rows) and t.size(1) and t.is_contiguous()):
+        return t
+    t = _i32(t, (rows, None), device, "page_table")
+    if t.size(1) < 1:
+        raise ValueError(f"page_table must have a column, got shape {tuple(t.shape)}")
+    return t
+
+
 def _operand(t: torch.Tensor) -> tuple:
-    """A [B, H, N, d] operand and the strides to pass for it: the tensor where
-    it lies, unless the channels are not next to each other or every stride
+    """A [B, H, N, d] operand and the strides to pass for it (None: contiguous):
+    the tensor where it lies, unless the channels are not next to each other or every stride
     is 0 (the C ABI's mark for a contiguous tensor)."""
     if t.is_contiguous():
-        return t, (0, 0, 0)
+        return t, None
     if (t.size(-1) > 1 and t.stride(-1) != 1) or not any(ops.strides_of(t)):
-        t = t.contiguous()
-        return t, (0, 0, 0)
+        return t.contiguous(), None
     return t, ops.strides_of(t)
+
+
+def _stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _no_grad(*ts) -> None:
@@ -112,6 +129,9 @@ class QuantizedKVCache:
         self._c = c
         self.num_pages, self.kv_heads = c.pages, c.kv_heads
         self.page_size, self.head_dim = c.page_size, c.head_dim
+        self.device = k_codes.device
+        self._ref = ctypes.byref(c)
+        self._workspaces = {}  # bytes by call shape
 
     @classmethod
     def from_tensors(cls, k_codes, k_params, v_codes, v_params, head_dim: int) -> "QuantizedKVCache":
@@ -144,10 +164,6 @@ class QuantizedKVCache:
         self = cls.__new__(cls)
         self._hold(c, k_codes, k_params, v_codes, v_params)
         return self
-
-    @property
-    def device(self) -> torch.device:
-        return self.k_codes.device
 
     def nbytes(self) -> int:
         """Bytes of the pool."""
@@ -192,6 +208,12 @@ class QuantizedKVCache:
 
 
 def check_tokens(cache, K, V) -> None:
+    if (type(K) is torch.Tensor and type(V) is torch.Tensor and K.dtype in ops.INPUT_DTYPES
+            and V.dtype is K.dtype and K.dim() == 4 and V.shape == K.shape and K.numel()
+            and K.size(1) == cache.kv_heads and K.size(3) == cache.head_dim
+            and K.is_cuda and K.device == cache.device and V.device == cache.device
+            and not (K.requires_grad or V.requires_grad)):
+        return
     for name, t in (("K", K), ("V", V)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a tensor")
@@ -222,18 +244,20 @@ def write_tokens(cache, K, V, page_table, start, counts=None) -> None:
     check_tokens(cache, K, V)
     dev = cache.device
     B, _, n, _ = K.shape
-    table = _i32(page_table, (B, None), dev, "page_table")
+    table = _table(page_table, B, dev)
     start = _i32(start, (B,), dev, "start")
     counts = None if counts is None else _i32(counts, (B,), dev, "counts")
     K, ks = _operand(K)
     V, vs = _operand(V)
     t = _lib.CacheTokens(B, n, ops._DTYPES[K.dtype], table.size(1), table.data_ptr(), start.data_ptr())
-    t.k_strides[:] = ks
-    t.v_strides[:] = vs
+    if ks:
+        t.k_strides[:] = ks
+    if vs:
+        t.v_strides[:] = vs
     with ops._on_device(dev):
-        rc = _lib.load().asa_cache_write(ctypes.byref(cache._c), ctypes.byref(t),
+        rc = _lib.load().asa_cache_write(cache._ref, ctypes.byref(t),
                                          None if counts is None else counts.data_ptr(), K.data_ptr(),
-                                         V.data_ptr(), ops._stream(dev))
+                                         V.data_ptr(), _stream(dev))
     _lib.check(rc)
 
 
@@ -243,7 +267,7 @@ def read_tokens(cache, page_table, lengths, n=None, dtype=torch.bfloat16, start=
         raise TypeError(f"unsupported dtype {dtype}; use torch.float32, torch.bfloat16 "
                         "or torch.float16")
     dev = cache.device
-    table = _i32(page_table, (None, None), dev, "page_table")
+    table = _table(page_table, None, dev)
     B = table.size(0)
     n = table.size(1) * cache.page_size if n is None else int(n)
     if B < 1 or n < 1:
@@ -255,13 +279,18 @@ def read_tokens(cache, page_table, lengths, n=None, dtype=torch.bfloat16, start=
     t = _lib.CacheTokens(B, n, ops._DTYPES[dtype], table.size(1), table.data_ptr(),
                          None if start is None else start.data_ptr())
     with ops._on_device(dev):
-        rc = _lib.load().asa_cache_read(ctypes.byref(cache._c), ctypes.byref(t), lengths.data_ptr(),
-                                        K.data_ptr(), V.data_ptr(), ops._stream(dev))
+        rc = _lib.load().asa_cache_read(cache._ref, ctypes.byref(t), lengths.data_ptr(),
+                                        K.data_ptr(), V.data_ptr(), _stream(dev))
     _lib.check(rc)
     return K, V
 
 
 def check_query(cache, Q, max_length=None) -> None:
+    if (type(Q) is torch.Tensor and type(cache) is QuantizedKVCache and max_length is None
+            and Q.dtype in ops.INPUT_DTYPES and Q.dim() == 4 and Q.numel()
+            and Q.size(3) == cache.head_dim and Q.size(1) % cache.kv_heads == 0
+            and Q.size(2) <= MAX_QUERIES and Q.is_cuda and Q.device == cache.device and not Q.requires_grad):
+        return
     if not isinstance(cache, QuantizedKVCache):
         raise TypeError("cache must be a QuantizedKVCache")
     if not isinstance(Q, torch.Tensor):
@@ -296,22 +325,29 @@ def attend(cache, Q, page_table, lengths, Q_idx, alpha: float, sm_scale: float,
     check_query(cache, Q, max_length)
     lib, dev = _lib.load(), cache.device
     B, H, NQ, d = Q.shape
-    table = _i32(page_table, (B, None), dev, "page_table")
+    table = _table(page_table, B, dev)
     lengths = _i32(lengths, (B,), dev, "lengths")
     Q_idx = None if Q_idx is None else _i32(Q_idx, (B, NQ), dev, "Q_idx")
     Q, qs = _operand(Q)
-    out = torch.empty((B, H, NQ, d), dtype=Q.dtype, device=dev)
-    a = _lib.CacheQuery(B, H, NQ, ops._DTYPES[Q.dtype], table.size(1),
-                        0 if max_length is None else min(int(max_length), 2 ** 31 - 1), alpha,
-                        sm_scale, table.data_ptr(), lengths.data_ptr(),
-                        None if Q_idx is None else Q_idx.data_ptr())
-    a.q_strides[:] = qs
-    c, need = ctypes.byref(cache._c), ctypes.c_size_t()
+    out = torch.empty_like(Q, memory_format=torch.contiguous_format)
+    P = table.size(1)
+    most = 0 if max_length is None else min(int(max_length), 2 ** 31 - 1)
+    dtype = ops._DTYPES[Q.dtype]
+    a = _lib.CacheQuery(B, H, NQ, dtype, P, most, alpha, sm_scale, table.data_ptr(),
+                        lengths.data_ptr(), None if Q_idx is None else Q_idx.data_ptr())
+    if qs:
+        a.q_strides[:] = qs
+    ref = ctypes.byref(a)
+    key = (B, H, NQ, dtype, P, most)
     with ops._on_device(dev):
-        _lib.check(lib.asa_cache_attention_workspace(c, ctypes.byref(a), ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        rc = lib.asa_cache_attention(c, ctypes.byref(a), Q.data_ptr(), out.data_ptr(),
-                                     None if ws is None else ws.data_ptr(), ops._stream(dev))
+        need = cache._workspaces.get(key)
+        if need is None:
+            z = ctypes.c_size_t()
+            _lib.check(lib.asa_cache_attention_workspace(cache._ref, ref, ctypes.byref(z)))
+            need = cache._workspaces[key] = z.value
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        rc = lib.asa_cache_attention(cache._ref, ref, Q.data_ptr(), out.data_ptr(),
+                                     None if ws is None else ws.data_ptr(), _stream(dev))
     _lib.check(rc)
     return out
 
