@@ -98,7 +98,7 @@ enum CachePlan : int { kCacheOneBlock = 0, kCacheSplit = 1 };
 // Keys whose maxima are kept together, and the static LDS of a one-block
 // kernel beside its dots (an upper bound).
 constexpr int kCacheGranule = 64;
-constexpr size_t kCacheOneStatic = 32768;
+constexpr size_t kCacheOneStatic = 45056;
 // One-block plan: dynamic LDS bytes, and the keys of a row there.
 inline size_t cache_one_lds(const CacheAttnParams& p, int* stride) {
   const int rows = p.R < p.tile_rows ? p.R : p.tile_rows;

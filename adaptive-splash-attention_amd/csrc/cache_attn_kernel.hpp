@@ -451,14 +451,16 @@ template <int PC> __device__ __forceinline__ void powers(float v, float e, float
   }
 }
 
-// The next tau from tau, where F = sum v^e and F1 = sum v^(e-1) over the
-// keys with v = z - tau > 0; true when tau is final.  For alpha <= 2 (e >= 1)
-// the step is Newton's on the norm F^(1/e) - 1: the norm is convex in tau and
+// One step from tau, where F = sum v^e and F1 = sum v^(e-1) over the keys with
+// v = z - tau > 0; true if tau is final instead.  For alpha <= 2 (e >= 1) the
+// step is Newton's on the norm F^(1/e) - 1: the norm is convex in tau and
 // nearly straight, so the steps from the left end stay left of the root and
-// few are needed.  For alpha > 2 a key just above tau makes F1 unbounded, and
-// the bracket is halved instead.
+// few are needed (five or six from max z - 1).  For alpha > 2 a key just above
+// tau makes F1 unbounded, and the bracket is halved instead.  |F - 1| <= 5e-7
+// is a few roundings of the sum; the weights are divided by it anyway.
 __device__ __forceinline__ bool next_tau(float alpha, float F, float F1, float& tau, float& lo, float& hi) {
   const float f = F - 1.0f;
+  if (fabsf(f) <= 5e-7f) return true;
   if (f >= 0.0f) lo = tau;
   else hi = tau;
   float nt = 0.5f * (lo + hi);
@@ -466,9 +468,9 @@ __device__ __forceinline__ bool next_tau(float alpha, float F, float F1, float& 
     const float s = tau + (F - __builtin_amdgcn_exp2f((2.0f - alpha) * __builtin_amdgcn_logf(F))) * __builtin_amdgcn_rcpf(F1);
     if (s >= lo && s <= hi) nt = s;
   }
-  const bool done = nt == tau || nt == lo || fabsf(f) <= (alpha <= 2.0f ? 1e-6f : 1e-7f);
-  if (alpha <= 2.0f || !done) tau = nt;
-  return done;
+  if (nt == tau || nt == lo || nt == hi) return true;  // between neighbouring floats
+  tau = nt;
+  return false;
 }
 constexpr int kMaxSteps = 64;
 
@@ -493,19 +495,19 @@ __device__ __forceinline__ int slot_of(const CacheAttnParams& p, int b, int key)
   return pg >= 0 && pg < p.c.pages ? (pg << p.c.page_shift) + (key & (p.c.page - 1)) : -1;
 }
 
-// Adds p_j v_j of the wave's listed keys to the lane's 8 channels: CL lanes
-// have a row's octets, so four loads in flight take 4 * 64 / CL entries.
-template <int NG>
+// Adds p_j v_j of the wave's listed keys to the lane's 8 channels: kCl lanes
+// have a row's octets, so DEEP loads in flight take DEEP * 64 / kCl entries.
+template <int NG, int DEEP>
 struct ValueSum {
-  static constexpr int kCl = NG == 3 ? 16 : 4 * NG, kPer = kWave / kCl, kStep = 4 * kPer;
+  static constexpr int kCl = NG == 3 ? 16 : 4 * NG, kPer = kWave / kCl, kDeep = DEEP, kStep = kDeep * kPer;
   float acc[8] = {};
   float off = 0.0f;
-  uint32_t w[4], pr[4];
+  uint32_t w[kDeep], pr[kDeep];
   // entries e0 .. of a list of slots (slot_of; -1: no row)
   __device__ __forceinline__ void load(const CacheAttnParams& p, int h, const int* pi, int e0, int n, int lane) {
     const int c = lane & (kCl - 1), slot = lane / kCl, g = c >> 2;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kDeep; ++u) {
       const int e = e0 + u * kPer + slot;
       const int at = e < n && g < NG ? pi[e] : -1;
       w[u] = pr[u] = 0u;
@@ -520,7 +522,7 @@ struct ValueSum {
   __device__ __forceinline__ void use(const float* pz, int e0, int n, int lane) {
     const int slot = lane / kCl;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kDeep; ++u) {
       const int e = e0 + u * kPer + slot;
       const float pj = e < n ? pz[e] : 0.0f;
       const float ps = pj * __uint_as_float(pr[u] << 16);
@@ -538,7 +540,7 @@ struct ValueSum {
     if (n > 0) next.load(p, h, pi, 0, n, lane);
     for (int e0 = 0; e0 < n; e0 += kStep) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) w[u] = next.w[u], pr[u] = next.pr[u];
+      for (int u = 0; u < kDeep; ++u) w[u] = next.w[u], pr[u] = next.pr[u];
       if (e0 + kStep < n) next.load(p, h, pi, e0 + kStep, n, lane);
       use(pz, e0, n, lane);
     }
@@ -575,9 +577,20 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
   // granule i is member i % size's
   const int ng = (vis + kGranule - 1) / kGranule;
   const int g0 = lane * size + member;
-  const float gfirst = g0 < ng ? zof(gp[g0]) : kHidden;
-  float g = gfirst;
-  for (int i = g0 + size * kWave; i < ng; i += size * kWave) g = fmaxf(g, zof(gp[i]));
+  constexpr int kHeld = WHOLE ? 4 : 1;  // granules of a lane whose maxima stay in registers
+  constexpr int kDeep = WHOLE ? 8 : 4;  // loads in flight of a wave: global memory, LDS
+  float held[kHeld];
+#pragma unroll
+  for (int c = 0; c < kHeld; ++c) {
+    const int i = g0 + c * size * kWave;
+    held[c] = i < ng ? gp[i] : kHidden;
+  }
+#pragma unroll
+  for (int c = 0; c < kHeld; ++c) held[c] = zof(held[c]);
+  float g = held[0];
+#pragma unroll
+  for (int c = 1; c < kHeld; ++c) g = fmaxf(g, held[c]);
+  for (int i = g0 + kHeld * size * kWave; i < ng; i += size * kWave) g = fmaxf(g, zof(gp[i]));
   L.gm[w][lane] = g;
   __syncthreads();
   if (member == 0) {
@@ -633,25 +646,27 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
         }
         mine += __builtin_popcountll(m);
       };
-      for (int i0 = 0; i0 < ng; i0 += size * kWave) {
-        const int i = i0 + g0;
-        uint64_t todo = __ballot(i < ng && (i0 ? zof(gp[i < ng ? i : 0]) : gfirst) > lo);
-        while (todo) {
-          constexpr int kDeep = 8;  // granules in flight
-          float d[kDeep];
-          int key[kDeep];
+      for (int i0 = 0; i0 < ng; i0 += kHeld * size * kWave) {
 #pragma unroll
-          for (int k = 0; k < kDeep; ++k) {
-            const int l = todo ? __builtin_ctzll(todo) : -1;
-            todo &= todo - 1;
-            const int gi = l < 0 ? 0 : i0 + l * size + member;
-            key[k] = l < 0 ? vis : gi * kGranule + lane;
-            d[k] = kHidden;
-            if (l >= 0) d[k] = sp[size_t(gi) * gstep + lane];
+        for (int c = 0; c < kHeld; ++c) {
+          const int i1 = i0 + c * size * kWave;
+          // the granules to look at, as a mask of the lanes that have them
+          uint64_t todo = __ballot((i0 ? (i1 + g0 < ng ? zof(gp[i1 + g0]) : kHidden) : held[c]) > lo);
+          while (todo) {
+            float d[kDeep];
+            int key[kDeep];
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+              const int l = todo ? __builtin_ctzll(todo) : -1;
+              todo &= todo - 1;
+              const int gi = l < 0 ? 0 : i1 + l * size + member;
+              key[k] = l < 0 ? vis : gi * kGranule + lane;
+              d[k] = kHidden;
+              if (l >= 0) d[k] = sp[size_t(gi) * gstep + lane];
+            }
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) collect(d[k], key[k]);
           }
-#pragma unroll
-          for (int k = 0; k < kDeep; ++k)
-            collect(d[k], key[k]);
         }
       }
       if (lane == 0) L.cnt[w] = mine;
@@ -694,8 +709,9 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
   }
 
   // ---- tau over the lists ----
-  ValueSum<NG> vs;
-  const bool few = listed && mine <= ValueSum<NG>::kStep;
+  using Values = ValueSum<NG, kDeep>;
+  Values vs;
+  const bool few = listed && mine <= Values::kStep;
   if (few) {
     for (int j = lane; j < mine; j += kWave) L.ci[w][j] = slot_of(p, b, L.ci[w][j]);
     vs.load(p, h, L.ci[w], 0, mine, lane);
@@ -703,7 +719,6 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
   float total = 0.0f;
   if (WHOLE && listed && most > kWave) {  // each wave its own
     tau = lo;
-    bool done = false;
     for (int it = 0; it <= kMaxSteps; ++it) {
       float F = 0.0f, F1 = 0.0f;
 #pragma unroll 2
@@ -719,42 +734,44 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
         L.red[it & 1][w][1] = F1;
       }
       __syncthreads();
-      total = F1 = 0.0f;
-      for (int i = 0; i < NW; ++i) {
-        total += L.red[it & 1][i][0];
-        F1 += L.red[it & 1][i][1];
-      }
-      if (done || it == kMaxSteps) break;  // the sum at the final tau
-      done = next_tau(p.alpha, total, F1, tau, lo, hi);
+      F = lane < NW ? L.red[it & 1][lane][0] : 0.0f;
+      F1 = lane < NW ? L.red[it & 1][lane][1] : 0.0f;
+      wave_sum2(F, F1);
+      total = F;
+      if (next_tau(p.alpha, F, F1, tau, lo, hi)) break;
     }
     __syncthreads();
   } else {
     if (listed && member == 0) {
       float t = lo;
-      bool done = false;
       auto steps = [&](auto sums) {
         for (int it = 0; it <= kMaxSteps; ++it) {
           float F = 0.0f, F1 = 0.0f;
           sums(t, F, F1);
           wave_sum2(F, F1);
           total = F;
-          if (done || it == kMaxSteps) break;
-          done = next_tau(p.alpha, total, F1, t, lo, hi);
+          if (next_tau(p.alpha, F, F1, t, lo, hi)) break;
         }
       };
       if (most <= kWave) {  // a register for each wave's list
         float z[NW];
+        int cnt[NW];
 #pragma unroll
-        for (int i = 0; i < NW; ++i) z[i] = i < size && lane < L.cnt[w + i] ? L.cz[w + i][lane] : kHidden;
+        for (int i = 0; i < NW; ++i) {
+          const int j = i < size ? w + i : w;
+          cnt[i] = L.cnt[j];
+          z[i] = L.cz[j][lane];
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i) z[i] = i < size && lane < cnt[i] ? z[i] : kHidden;
         steps([&](float at, float& F, float& F1) {
 #pragma unroll
-          for (int i = 0; i < NW; ++i)
-            if (i < size) {
-              float pa, pa1;
-              powers<PC>(fmaxf(z[i] - at, 0.0f), e, pa, pa1);
-              F += pa;
-              F1 += pa1;
-            }
+          for (int i = 0; i < NW; ++i) {
+            float pa, pa1;
+            powers<PC>(fmaxf(z[i] - at, 0.0f), e, pa, pa1);
+            F += pa;
+            F1 += pa1;
+          }
         });
       } else {
         steps([&](float at, float& F, float& F1) {
@@ -819,7 +836,7 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
     }
   }
   vs.reduce();
-  if (lane < ValueSum<NG>::kCl && lane < 4 * NG)
+  if (lane < Values::kCl && lane < 4 * NG)
     for (int j = 0; j < 8; ++j) L.acc[w][8 * lane + j] = vs.acc[j];
   if (!listed) {
     psum = wave_sum(psum);
@@ -849,11 +866,11 @@ constexpr int kScoreWaves = 4;  // split plan: score blocks
 constexpr int kRowKeys = 8192;  // split plan: rows up to this have 4 waves, else 8 or 16
 
 // One block per tile of rows of a key head: dots into LDS, then its rows.
-using OneLds = TeamLds<kOneWaves, 128>;
 template <typename T, int P, int NG, int PC>
 __global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnParams p, int stride) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ OneLds L;
+  constexpr int NW = kOneWaves;
+  __shared__ TeamLds<NW, 128> L;
   constexpr int kR = kTile / P;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   const int nrt = (p.R + kR - 1) / kR;
@@ -861,26 +878,26 @@ __global__ __launch_bounds__(kOneWaves * kWave) void cache_one_kernel(CacheAttnP
   const int b = bh / p.c.heads, h = bh % p.c.heads;
   const int r0 = tile * kR, rows = min(kR, p.R - r0), most = min(kR, p.R), gs = stride / kGranule;
   int pad = 1;
-  while (pad < most && pad < kOneWaves) pad *= 2;
+  while (pad < most && pad < NW) pad *= 2;
   float* zs = reinterpret_cast<float*>(smem);
   float* gs0 = zs + most * stride;  // granule maxima
   int* pages = reinterpret_cast<int*>(gs0 + most * gs);
-  stage_pages(p, b, 0, p.maxlen, pages, t, kOneWaves * kWave);
+  stage_pages(p, b, 0, p.maxlen, pages, t, NW * kWave);
   __shared__ QueryLds<T, P, NG> ql;
   static_assert(sizeof(L) + sizeof(ql) <= kCacheOneStatic, "the plan's bound");
-  stage_query<T, P, NG>(p, ql, b, h, r0, w, kOneWaves, lane);
+  stage_query<T, P, NG>(p, ql, b, h, r0, w, NW, lane);
   {
     TileRows<P> rt;
     rt.load(p, b, r0, lane);
     __syncthreads();
-    score_keys<kOneWaves, false>(p, ql, rt, h, 0, rt.most, pages, most, zs, gs0, gs, w, lane);
+    score_keys<NW, false>(p, ql, rt, h, 0, rt.most, pages, most, zs, gs0, gs, w, lane);
   }
   __syncthreads();
-  const int size = kOneWaves / pad, team = w / size, w0 = team * size;
+  const int size = NW / pad, team = w / size, w0 = team * size;
   for (int first = 0; first < rows; first += pad) {
     const int r = first + team;
     const bool has = r < rows;
-    finish_row<T, NG, PC, kOneWaves, false>(p, b, h, has ? r0 + r : -1, has ? visible_keys(p, b, (r0 + r) % p.NQ) : 0,
+    finish_row<T, NG, PC, NW, false>(p, b, h, has ? r0 + r : -1, has ? visible_keys(p, b, (r0 + r) % p.NQ) : 0,
                                         gs0 + (has ? r : 0) * gs, zs + (has ? r : 0) * kGranule, most * kGranule, L, w,
                                         w0, size, lane);
   }
@@ -916,7 +933,7 @@ __global__ __launch_bounds__(kScoreWaves * kWave, 4) void cache_score_kernel(Cac
 // Split plan, second launch: one block per row.
 template <typename T, int NG, int PC, int NW>
 __global__ __launch_bounds__(NW * kWave) void cache_row_kernel(CacheAttnParams p) {
-  __shared__ TeamLds<NW, NW == 16 ? 256 : 512> L;
+  __shared__ TeamLds<NW, 512> L;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63;
   const int row = blockIdx.x % p.R, bh = blockIdx.x / p.R;
   const int b = bh / p.c.heads, h = bh % p.c.heads;
@@ -942,7 +959,8 @@ hipError_t launch_png(const CacheAttnParams& p, hipStream_t s) {
     auto kern = p.pc == kE2 ? cache_one_kernel<T, P, NG, kE2> : cache_one_kernel<T, P, NG, kEGen>;
     if (hipError_t e = allow_lds(kern, lds)) return e;
     profile_begin("cache_attn", s);
-    hipLaunchKernelGGL(kern, dim3(unsigned(p.B) * p.c.heads * nrt), dim3(kOneWaves * kWave), lds, s, p, stride);
+    hipLaunchKernelGGL(kern, dim3(unsigned(p.B) * p.c.heads * nrt), dim3(kOneWaves * kWave), lds, s, p,
+                       stride);
     profile_end(s);
     return hipGetLastError();
   }
