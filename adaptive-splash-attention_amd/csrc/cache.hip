@@ -65,24 +65,30 @@ __device__ __forceinline__ void two_diff(float a, float b, float& hi, float& lo)
   lo = (a - (hi - t)) - (b + t);
 }
 
-// The codes (nibble j: channel j) and the group's params of 8 channels x, of
-// which nv belong to the row.  Called by whole quads: a quad is a group.
-__device__ __forceinline__ uint32_t quantise8(float* x, int nv, uint32_t& params) {
+// The codes (nibble j of dword i: channel 8 i + j) and the group's params of N
+// channels x, of which nv belong to the row (FULL: all).  Called by whole
+// quads (N = 8) or pairs (N = 16): the lanes of a group.
+template <int N, bool FULL>
+__device__ __forceinline__ void quantise(float* x, int nv, uint32_t& params, uint32_t* codes) {
   bool wild = false;
-  for (int j = 0; j < 8; ++j) wild |= !(fabsf(x[j]) <= kMostCached);
+  for (int j = 0; j < N; ++j) wild |= !(fabsf(x[j]) <= kMostCached);
   if (wild)
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < N; ++j)
       x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -kMostCached), kMostCached) : 0.0f;
   float lo = __builtin_inff(), hi = -__builtin_inff();
-  for (int j = 0; j < 8; ++j)
-    if (j < nv) {
+  for (int j = 0; j < N; ++j)
+    if (FULL || j < nv) {
       lo = fminf(lo, x[j]);
       hi = fmaxf(hi, x[j]);
     }
   lo = fminf(lo, __uint_as_float(lane_xor<1>(__float_as_uint(lo))));
   hi = fmaxf(hi, __uint_as_float(lane_xor<1>(__float_as_uint(hi))));
-  lo = fminf(lo, __uint_as_float(lane_xor<2>(__float_as_uint(lo))));
-  hi = fmaxf(hi, __uint_as_float(lane_xor<2>(__float_as_uint(hi))));
+  if constexpr (N == 8) {
+    lo = fminf(lo, __uint_as_float(lane_xor<2>(__float_as_uint(lo))));
+    hi = fmaxf(hi, __uint_as_float(lane_xor<2>(__float_as_uint(hi))));
+  }
+  if constexpr (!FULL)
+    for (int j = 0; j < N; ++j) x[j] = j < nv ? x[j] : lo;  // code 0 or 1, cleared below
   // m: towards zero in the bits, one step further down for a cut negative
   const uint32_t lb = __float_as_uint(lo);
   const uint32_t mb = (lb & 0xffff0000u) + (lo < 0.0f && (lb & 0xffffu) ? 0x10000u : 0u);
@@ -106,40 +112,55 @@ __device__ __forceinline__ uint32_t quantise8(float* x, int nv, uint32_t& params
   // settles the code whatever y was rounded to.
   const float r = sb ? __builtin_amdgcn_rcpf(s) : 0.0f;
   const float nm = -m * r;
-  uint32_t w = 0u;
   // m + (k + 1/2) s: m is a multiple of 2^-7 of its power of two and the rest
   // of 2^-8 of s's, so between |m| = 2^-8 s and 2^12 s the sum spans at most
   // 22 bits and the fused product rounds nothing.
   const float am = fabsf(m);
   if (am == 0.0f || (am >= 0x1p-8f * s && am <= 0x1p12f * s)) {
-    for (int j = 7; j >= 0; --j) {
-      const float k = floorf(fmaf(x[j], r, nm));
-      const float border = fmaf(k + 0.5f, s, m);
-      const int c = int(k) + (x[j] > border ? 1 : 0);
-      w = (w << 4) | uint32_t(c);
+    for (int i = 0; i < N / 8; ++i) {
+      // four codes at a time gather in a float (16 bits, exact)
+      float half[2];
+      for (int q = 0; q < 2; ++q) {
+        float acc = 0.0f;
+        for (int j = 3; j >= 0; --j) {
+          const float v = x[8 * i + 4 * q + j];
+          const float k = floorf(fmaf(v, r, nm)), k5 = k + 0.5f;
+          acc = fmaf(acc, 16.0f, v > fmaf(k5, s, m) ? k5 + 0.5f : k);
+        }
+        half[q] = acc;
+      }
+      codes[i] = uint32_t(half[0]) | (uint32_t(half[1]) << 16);
     }
   } else {
-    for (int j = 7; j >= 0; --j) {
-      float t, tl;
-      two_diff(x[j], m, t, tl);
-      const float k = fminf(fmaxf(floorf(t * r), 0.0f), 15.0f);
-      const float border = (k + 0.5f) * s;
-      const int c = int(k) + (t > border || (t == border && tl > 0.0f) ? 1 : 0);
-      w = (w << 4) | uint32_t(c > 15 ? 15 : c);
+    for (int i = 0; i < N / 8; ++i) {
+      uint32_t w = 0u;
+      for (int j = 7; j >= 0; --j) {
+        float t, tl;
+        two_diff(x[8 * i + j], m, t, tl);
+        const float k = fminf(fmaxf(floorf(t * r), 0.0f), 15.0f);
+        const float border = (k + 0.5f) * s;
+        const int c = int(k) + (t > border || (t == border && tl > 0.0f) ? 1 : 0);
+        w = (w << 4) | uint32_t(c > 15 ? 15 : c);
+      }
+      codes[i] = w;
     }
   }
-  if (nv < 8) w = nv <= 0 ? 0u : w & (0xffffffffu >> (4 * (8 - nv)));
-  return w;
+  if constexpr (!FULL)
+    if (nv < 8) codes[0] = nv <= 0 ? 0u : codes[0] & (0xffffffffu >> (4 * (8 - nv)));
 }
 
-template <typename T, bool CHUNKS>
+// N = 16: rows are whole channel groups of 16-byte chunks, and a thread has
+// half a group; N = 8: a quarter, whatever the row.
+template <typename T, int N, bool CHUNKS>
 __global__ __launch_bounds__(kThreads) void cache_write_kernel(CacheRowsParams p, int lanes_shift, int nblk) {
+  constexpr bool kFull = N == 16;
+  constexpr int kPer = 32 / N;  // threads of a group
   const int bh = blockIdx.x / nblk, b = bh / p.c.heads, h = bh % p.c.heads;
   const int t = (blockIdx.x - bh * nblk) * kThreads + threadIdx.x;
   const int i = t >> lanes_shift, l = t & ((1 << lanes_shift) - 1);
-  const int g = l >> 2, o = l & 3;
+  const int g = l / kPer, o = l % kPer * (N / 8);  // group, first octet
   const int count = p.limit ? min(p.limit[b], p.n) : p.n;
-  if (i >= count || g >= p.c.G) return;  // whole quads leave together
+  if (i >= count || g >= p.c.G) return;  // whole groups leave together
   const int64_t pos = int64_t(p.start ? p.start[b] : 0) + i;
   if (pos < 0 || pos >= (int64_t(1) << 31)) return;
   const int64_t row = cache_row(p.c, p.table + size_t(b) * p.cols, p.cols, int(pos), h);
@@ -147,17 +168,22 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(CacheRowsParams p
   const int ch = 32 * g + 8 * o, nv = p.c.hd - ch;
   const T* k = static_cast<const T*>(p.k) + size_t(b) * p.lk.sb + size_t(h) * p.lk.sh + size_t(i) * p.lk.sn + ch;
   const T* v = static_cast<const T*>(p.v) + size_t(b) * p.lv.sb + size_t(h) * p.lv.sh + size_t(i) * p.lv.sn + ch;
-  float xk[8] = {}, xv[8] = {};
-  if (nv > 0) {  // rows that end inside the group: its last octets have no channels
-    load8<T, CHUNKS>(k, nv, xk);
-    load8<T, CHUNKS>(v, nv, xv);
-  }
-  uint32_t pk, pv;
-  const uint32_t wk = quantise8(xk, nv, pk);
-  const uint32_t wv = quantise8(xv, nv, pv);
+  float xk[N] = {}, xv[N] = {};
+  if (kFull || nv > 0)  // rows that end inside the group: its last octets have no channels
+    for (int q = 0; q < N; q += 8) {
+      load8<T, CHUNKS>(k + q, nv, xk + q);
+      load8<T, CHUNKS>(v + q, nv, xv + q);
+    }
+  uint32_t pk, pv, wk[N / 8], wv[N / 8];
+  quantise<N, kFull>(xk, nv, pk, wk);
+  quantise<N, kFull>(xv, nv, pv, wv);
   const int G = p.c.G;
-  reinterpret_cast<uint32_t*>(p.c.k_codes)[row * (4 * G) + G * o + g] = wk;
-  reinterpret_cast<uint32_t*>(p.c.v_codes)[row * (4 * G) + 4 * g + o] = wv;
+  uint32_t* kc = reinterpret_cast<uint32_t*>(p.c.k_codes) + row * (4 * G) + G * o + g;
+  uint32_t* vc = reinterpret_cast<uint32_t*>(p.c.v_codes) + row * (4 * G) + 4 * g + o;
+  for (int q = 0; q < N / 8; ++q) {
+    kc[G * q] = wk[q];
+    vc[q] = wv[q];
+  }
   if (o == 0) {
     p.c.k_params[row * G + g] = pk;
     p.c.v_params[row * G + g] = pv;
@@ -197,23 +223,23 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(CacheRowsParams p,
   store8<T, CHUNKS>(static_cast<T*>(p.ov) + at, nv, xv);
 }
 
-// Threads of a row: 4 per channel group, rounded up to a power of two.
-int lanes_shift_of(int G) { return G > 2 ? 4 : G > 1 ? 3 : 2; }
-
 template <typename T>
 hipError_t launch_rows(const CacheRowsParams& p, bool write, hipStream_t s) {
-  const int sh = lanes_shift_of(p.c.G);
+  // threads of a row, rounded up to a power of two: 2 or 4 per channel group
+  const bool halves = write && p.chunks && p.c.hd % 32 == 0;
+  const int sh = (p.c.G > 2 ? 4 : p.c.G > 1 ? 3 : 2) - (halves ? 1 : 0);
   const long long threads = (long long)p.n << sh;
   const long long nblk = (threads + kThreads - 1) / kThreads;
   const long long blocks = nblk * p.B * p.c.heads;
   if (threads >= (1LL << 31) || blocks >= (1LL << 31)) return hipErrorInvalidConfiguration;
-  const dim3 grid{unsigned(blocks)};
+  const dim3 grid{unsigned(blocks)}, block(kThreads);
   if (write) {
-    if (p.chunks) hipLaunchKernelGGL((cache_write_kernel<T, true>), grid, dim3(kThreads), 0, s, p, sh, int(nblk));
-    else hipLaunchKernelGGL((cache_write_kernel<T, false>), grid, dim3(kThreads), 0, s, p, sh, int(nblk));
+    if (halves) hipLaunchKernelGGL((cache_write_kernel<T, 16, true>), grid, block, 0, s, p, sh, int(nblk));
+    else if (p.chunks) hipLaunchKernelGGL((cache_write_kernel<T, 8, true>), grid, block, 0, s, p, sh, int(nblk));
+    else hipLaunchKernelGGL((cache_write_kernel<T, 8, false>), grid, block, 0, s, p, sh, int(nblk));
   } else {
-    if (p.chunks) hipLaunchKernelGGL((cache_read_kernel<T, true>), grid, dim3(kThreads), 0, s, p, sh, int(nblk));
-    else hipLaunchKernelGGL((cache_read_kernel<T, false>), grid, dim3(kThreads), 0, s, p, sh, int(nblk));
+    if (p.chunks) hipLaunchKernelGGL((cache_read_kernel<T, true>), grid, block, 0, s, p, sh, int(nblk));
+    else hipLaunchKernelGGL((cache_read_kernel<T, false>), grid, block, 0, s, p, sh, int(nblk));
   }
   return hipGetLastError();
 }

@@ -14,14 +14,25 @@ size_t cache_attn_plan(CacheAttnParams& p, int dtype, size_t max_lds, int cus) {
   // possible share a result; fp32 queries (three operand reads of LDS for
   // each key tile) share two at most.
   p.tile_rows = p.R > 8 ? 16 : p.R > 4 || dtype == kElemF32 ? 8 : 4;
+  const long long nrt = (p.R + p.tile_rows - 1) / p.tile_rows, tiles = (long long)p.B * p.c.heads * nrt;
+  // One launch or two.  With a tile of rows for nearly every compute unit one
+  // block each is faster as long as two fit a unit's LDS (head dimension 128,
+  // four rows per key head, us with one launch / two: 256 tiles of 512 keys
+  // 13.4 / 17.7, of 4096 29.1 / 33.6; 1024 tiles of 2048 53 / 71).  Fewer
+  // tiles leave units idle that split keys would use (8 tiles of 2048 keys
+  // 17.1 / 11.7, 64 tiles 17.7 / 14.1), but the second launch is not made up
+  // for by few bytes of keys (8 tiles of 512: 11.4 / 11.5) unless a block has
+  // more rows than waves (16 rows, 8 tiles of 300: 18.5 / 13.1).
   int stride = 0;
+  const size_t lds = cache_one_lds(p, &stride);
   p.span = p.nsplit = 0;
-  if (p.maxlen <= 2048 && cache_one_lds(p, &stride) + kCacheOneStatic <= max_lds) {
+  const bool many = tiles >= cus * 3 / 4 && lds <= 72 * 1024;
+  const bool few = (long long)p.maxlen * p.c.G <= 2048 && p.R <= 8;
+  if ((many || few) && lds + kCacheOneStatic <= max_lds) {
     p.plan = kCacheOneBlock;
     return 0;
   }
   p.plan = kCacheSplit;
-  const long long nrt = (p.R + p.tile_rows - 1) / p.tile_rows, tiles = (long long)p.B * p.c.heads * nrt;
   // eight score blocks per compute unit, of at least 256 keys (the largest
   // page: a block starts on a page)
   long long span = (p.maxlen * tiles + 8LL * cus - 1) / (8LL * cus);
