@@ -3,21 +3,28 @@
 // Per query row, with z_j = (alpha - 1) clamp(scale q.k_j, -10, 10) over the
 // visible keys j and e = 1 / (alpha - 1):
 //
-//   sum_j max(z_j - tau, 0)^e = 1,  out = sum_j p_j v_j / sum_j p_j.
+//   sum_j max(z_j - tau, 0)^e = 1,  out = sum_j p_j v_j / sum_j p_j,
+//   p_j = max(z_j - tau, 0)^e.
 //
-// The keys' bytes are what a row costs: 5 bits per channel, read once.  The
-// codes never become keys.  With u = 16 + c (bf16 0x4180 | c << 3, exact),
-// group g and its query part q_g,
+// Bytes: the keys', 5 bits per channel, are what a row costs.  They are read
+// once and never become keys.  With u = 16 + c (exact in 16 bits: c is shifted
+// into the mantissa of 16.0), group g and its query part q_g,
 //
-//   q.k = sum_g s_g (q_g.u_g - 16 sum q_g) + sum_g m_g sum q_g:
+//   q.k = sum_g s_g (q_g.u_g - 16 sum q_g) + m_g sum q_g:
 //
-// one v_mfma_f32_16x16x32_bf16 per group gives q_g.u_g for 16 rows x 16 keys
-// (a group is the instruction's 32 channels), its accumulator starts at
-// -16 sum q_g, the keys' scales multiply the finished group sums (a lane of
-// the result holds one key, so G scales), and the offsets' part is one more
-// MFMA over the groups.  Queries enter as exact sums of bf16 terms (bf16 1,
-// fp16 2, fp32 3 terms), so that scores carry fp32 rounding only, for every
-// type.
+// one 16x16x32 MFMA per group gives q_g.u_g for 16 rows x 16 keys (a group is
+// the instruction's 32 channels), its accumulator starts at -16 sum q_g, and
+// the keys' scales multiply the finished group sums.  16-bit queries enter as
+// they are, fp32 ones as three bf16 terms (24 bits), so that scores carry
+// fp32 rounding only, for every type.
+//
+// A key head serves few query rows, and what follows an MFMA (scales, maxima,
+// stores) costs the same for one row as for 16.  With R <= 16 / P rows, P key
+// tiles share the 16 rows of one result: tile u's operand holds the queries
+// in rows u (16 / P) .. and zeros elsewhere, so that its products add to
+// those of the other tiles without meeting them, and each lane of the result
+// has a key of its own to scale (about 280 vector instructions per 64 keys of
+// head dimension 128 at P = 4, 600 before).
 //
 // tau lies in [max z - 1, max z], so only keys with z > max z - 1 can have a
 // weight.  A better bound: the sum over any part of the row is at most the
@@ -25,10 +32,19 @@
 // keys, which the score pass keeps) is at most tau, and close to it, since a
 // long row's support lies in as many granules.  Only granules whose maximum
 // is above that bound are looked at again: their keys above it are listed
-// (index, z) in LDS, Newton steps over the list find tau, and only the value
-// rows of the support are read.  alpha-entmax gives most keys of a long row
-// no weight, so the values' bytes are a small part of the keys'.  Lists have
-// a fixed order, so results do not depend on timing.
+// (key, z) in LDS, Newton steps over the list find tau, and only the value
+// rows of the list are read.  alpha-entmax gives most keys of a long row no
+// weight, so the values' bytes are a small part of the keys'.  A list that
+// does not fit raises the bound by Newton steps over the whole row, down to
+// rows with more weights than any list, which are summed as they are read.
+// Lists and sums have a fixed order: results do not depend on timing.
+//
+// Two plans (cache_attn_plan).  One block per tile of rows, dots in LDS; or
+// keys split over score blocks, dots in the workspace, then one block per
+// row.  16 x 32768 keys, 8 key heads, 32 heads of 128, bf16: score pass 75 us
+// for 335 MB of keys (the card reads 6.3 TB/s and copies 5.1; 61 MB of dots
+// are written), rows 15 us, which are latency: five dependent reads and a
+// dozen Newton steps.
 #pragma once
 
 #include <climits>
@@ -189,8 +205,20 @@ struct KeyGranule {
   bool seen[V];  // the lane's own key has a page
   bool whole;    // every key of the granule has one (wave-uniform)
 
+  // Where one tile holds all rows (P > 1: the plan's rule) the keys are read
+  // once in a call, and a large batch's would only push the dots and values
+  // out of the caches: 16 x 32768 93 -> 88 us, 4 x 16384 (spread rows) 47 ->
+  // 42, 1 x 131072 (84 MB, which do fit) 32 -> 33.
   template <int N> static __device__ __forceinline__ void words(uint32_t* d, const uint32_t* s) {
-    __builtin_memcpy(d, __builtin_assume_aligned(s, N == 4 ? 16 : N == 2 ? 8 : 4), 4 * N);
+    if constexpr (P > 1 && (N == 2 || N == 4)) {
+      typedef uint32_t vec __attribute__((ext_vector_type(N)));
+      const vec x = __builtin_nontemporal_load(reinterpret_cast<const vec*>(s));
+      __builtin_memcpy(d, &x, 4 * N);
+    } else if constexpr (P > 1) {
+      for (int i = 0; i < N; ++i) d[i] = __builtin_nontemporal_load(s + i);
+    } else {
+      __builtin_memcpy(d, __builtin_assume_aligned(s, N == 4 ? 16 : N == 2 ? 8 : 4), 4 * N);
+    }
   }
   // keys base .. base + 63 of [.., key1); pages: of the keys from key0
   __device__ __forceinline__ void load(const CachePool& c, int h, const int* pages, int key0, int base, int key1,
@@ -945,7 +973,7 @@ __global__ __launch_bounds__(NW * kWave) void cache_row_kernel(CacheAttnParams p
 }
 
 template <typename K> hipError_t allow_lds(K kern, size_t lds) {
-  if (lds <= 65536) return hipSuccess;
+  if (lds + kCacheOneStatic <= 65536) return hipSuccess;
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                              int(lds));
 }

@@ -373,9 +373,9 @@ int validate_tokens(const asa_cache* c, const asa_cache_tokens* t, asa::CacheRow
                 t->batch, t->n, t->max_pages);
   if (int rc = check_dtype(t->dtype)) return rc;
   if (!t->page_table) return fail(ASA_ERR_INVALID_ARGUMENT, "page_table is NULL");
-  // 16 threads per row at most, 256 to a block
-  const long long blocks = ((long long)t->n * 16 + 255) / 256;
-  if (t->n >= (1 << 26) || (long long)t->batch * c->kv_heads > ((1LL << 31) - 1) / blocks)
+  // a launch has less than 2^32 threads, 16 of them per row at most
+  if ((long long)t->n * 16 >= (1LL << 31) ||
+      (long long)t->batch * c->kv_heads >= (1LL << 32) / (((long long)t->n * 16 + 255) / 256 * 256))
     return fail(ASA_ERR_INVALID_ARGUMENT, "too many tokens in one call");
   rp->B = t->batch;
   rp->n = t->n;
@@ -407,7 +407,8 @@ int validate_query(const asa_cache* c, const asa_cache_query* a, bool pointers,
   if (most >= (1 << 28))
     return fail(ASA_ERR_INVALID_ARGUMENT, "max_length (%lld) must be below 2^28", most);
   const long long rows = (long long)a->batch * a->heads * a->nq;
-  if (rows >= (1LL << 24)) return fail(ASA_ERR_INVALID_ARGUMENT, "too many query rows (%lld)", rows);
+  // a launch has less than 2^32 threads, 1024 of them per row at most
+  if (rows >= (1LL << 22)) return fail(ASA_ERR_INVALID_ARGUMENT, "too many query rows (%lld)", rows);
   if (pointers && (!a->page_table || !a->lengths))
     return fail(ASA_ERR_INVALID_ARGUMENT, "page_table or lengths is NULL");
   ap->B = a->batch;
@@ -441,9 +442,10 @@ int plan_query(asa::CacheAttnParams* ap, int dtype, size_t* bytes) {
   }
   if (int rc = device_cus(&cus)) return rc;
   *bytes = asa::cache_attn_plan(*ap, dtype, size_t(max_lds), cus);
-  const long long blocks = (long long)ap->B * ap->c.heads * ((ap->R + 15) / 16) *
-                           (ap->nsplit > 1 ? ap->nsplit : 1);  // at least the launches' grids
-  if (blocks >= (1LL << 31)) return fail(ASA_ERR_INVALID_ARGUMENT, "problem too large");
+  const long long blocks = (long long)ap->B * ap->c.heads *
+                           ((ap->R + ap->tile_rows - 1) / ap->tile_rows) *
+                           (ap->nsplit > 1 ? ap->nsplit : 1);
+  if (blocks >= (1LL << 32) / 512) return fail(ASA_ERR_INVALID_ARGUMENT, "problem too large");
   return ASA_OK;
 }
 

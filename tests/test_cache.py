@@ -141,7 +141,7 @@ def test_c_entry_refuses_bad_caches(bad, msg):
 
 @pytest.mark.parametrize("bad,msg", [
     (dict(batch=0), "batch"), (dict(n=0), "n (0)"), (dict(max_pages=0), "max_pages"),
-    (dict(dtype=3), "dtype"), (dict(page_table=None), "page_table"), (dict(n=1 << 26), "too many"),
+    (dict(dtype=3), "dtype"), (dict(page_table=None), "page_table"), (dict(n=1 << 27), "too many"), (dict(n=1 << 20, batch=1 << 8), "too many"),
     (dict(k_strides=(0, -4, 64)), "k_strides[1]"),
 ])
 def test_c_entry_refuses_bad_tokens(bad, msg):
@@ -157,7 +157,7 @@ def test_c_entry_refuses_bad_tokens(bad, msg):
     (dict(batch=0), "batch"), (dict(heads=3), "multiple"), (dict(nq=0), "nq"), (dict(nq=65), "nq"),
     (dict(dtype=-1), "dtype"), (dict(alpha=float("nan")), "alpha"), (dict(sm_scale=float("inf")), "sm_scale"),
     (dict(max_length=-1), "max_length"), (dict(max_pages=1 << 25), "2^28"),
-    (dict(q_strides=(64, -1, 64)), "q_strides[1]"), (dict(batch=1 << 23), "too many"),
+    (dict(q_strides=(64, -1, 64)), "q_strides[1]"), (dict(batch=1 << 20), "too many"),
 ])
 def test_c_entry_refuses_bad_queries(bad, msg):
     lib, a = _lib.load(), 1 << 20

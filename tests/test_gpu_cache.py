@@ -457,6 +457,62 @@ def test_captured_steps_replay(dev, n):
         torch.zeros(1 << 20, device=dev).sum().item()
 
 
+@pytest.mark.parametrize("HK,rep,n", [(100, 4, 2500), (100, 16, 900), (200, 1, 5000)])
+def test_many_tiles_in_one_launch(dev, HK, rep, n):
+    """Enough tiles for one launch with long rows: dots past 64 KB of LDS,
+    captured and replayed, against the split of the same rows (few heads)."""
+    d = 32
+    c, table, L, k, v = filled(dev, [n, n - 70], HK, d, 64, torch.bfloat16, 21)
+    q = torch.randn(2, HK * rep, 1, d, device=dev).bfloat16()
+    out = c.attention(q, table, L)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        again = c.attention(q, table, L)
+    for _ in range(3):
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, out)
+        torch.zeros(1 << 18, device=dev).sum().item()
+    for h in (0, HK - 1):
+        check_attention(out[:, h * rep:(h + 1) * rep], q[:, h * rep:(h + 1) * rep], k[:, h:h + 1], v[:, h:h + 1],
+                        [n, n - 70], default_idx([n, n - 70], 1), 1.5, d ** -0.5)
+
+
+def test_two_threads_call_at_once(dev):
+    """Calls of one cache from two threads, each on a stream of its own."""
+    import threading
+
+    c, table, L, _, _ = filled(dev, [3000, 100], 2, 64, 32, torch.bfloat16, 22)
+    qs = [torch.randn(2, 4, n, 64, device=dev).bfloat16() for n in (1, 3)]
+    want = [c.attention(q, table, L) for q in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(c.attention(qs[i], table, L))
+            torch.cuda.current_stream().synchronize()
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    for g, w in zip(got, want):
+        assert len(g) == 20 and all(torch.equal(x, w) for x in g)
+
+
+def test_a_wide_page_table_of_short_sequences(dev):
+    """The table is as wide as the longest context that a server allows."""
+    c, table, L, k, v = filled(dev, [70, 3], 2, 64, 16, torch.float32, 23)
+    wide = torch.full((2, 8192), -1, dtype=torch.int32, device=dev)
+    wide[:, :table.size(1)] = table
+    q = torch.randn(2, 4, 1, 64, generator=torch.Generator().manual_seed(5))
+    check_attention(c.attention(q.to(dev), wide, L), q, k, v, [70, 3], [[69], [2]], 1.5, 0.125)
+    check_attention(c.attention(q.to(dev), wide, L, max_length=100), q, k, v, [70, 3], [[69], [2]], 1.5, 0.125)
+
+
 def test_compiled_steps(dev):
     """Through torch.compile, as custom operators, without a graph break."""
     c, table, L, _, _ = filled(dev, [100, 50], 2, 64, 16, torch.float32, 17)
