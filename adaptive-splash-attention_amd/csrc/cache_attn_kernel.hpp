@@ -681,10 +681,12 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
           // the granules to look at, as a mask of the lanes that have them
           uint64_t todo = __ballot((i0 ? (i1 + g0 < ng ? zof(gp[i1 + g0]) : kHidden) : held[c]) > lo);
           while (todo) {
-            float d[kDeep];
-            int key[kDeep];
+            constexpr int kLook = 2 * kDeep;
+            const int cnt = __builtin_popcountll(todo);
+            float d[kLook];
+            int key[kLook];
 #pragma unroll
-            for (int k = 0; k < kDeep; ++k) {
+            for (int k = 0; k < kLook; ++k) {
               const int l = todo ? __builtin_ctzll(todo) : -1;
               todo &= todo - 1;
               const int gi = l < 0 ? 0 : i1 + l * size + member;
@@ -693,7 +695,10 @@ __device__ __forceinline__ void finish_row(const CacheAttnParams& p, int b, int 
               if (l >= 0) d[k] = sp[size_t(gi) * gstep + lane];
             }
 #pragma unroll
-            for (int k = 0; k < kDeep; ++k) collect(d[k], key[k]);
+            for (int k = 0; k < kLook; ++k) {
+              if (k >= cnt) break;
+              collect(d[k], key[k]);
+            }
           }
         }
       }

@@ -60,8 +60,8 @@ def _table(t, rows, device) -> torch.Tensor:
 
 def _operand(t: torch.Tensor) -> tuple:
     """A [B, H, N, d] operand and the strides to pass for it (None: contiguous):
-    the tensor where it lies, unless the channels are not next to each other or every stride
-    is 0 (the C ABI's mark for a contiguous tensor)."""
+    the tensor where it lies, unless the channels are not next to each other
+    or every stride is 0 (the C ABI's mark for a contiguous tensor)."""
     if t.is_contiguous():
         return t, None
     if (t.size(-1) > 1 and t.stride(-1) != 1) or not any(ops.strides_of(t)):
@@ -71,6 +71,13 @@ def _operand(t: torch.Tensor) -> tuple:
 
 def _stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _on_device(dev: torch.device, fn, *args):
+    if torch.cuda.current_device() == dev.index:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
 
 
 def _no_grad(*ts) -> None:
@@ -254,11 +261,9 @@ def write_tokens(cache, K, V, page_table, start, counts=None) -> None:
         t.k_strides[:] = ks
     if vs:
         t.v_strides[:] = vs
-    with ops._on_device(dev):
-        rc = _lib.load().asa_cache_write(cache._ref, ctypes.byref(t),
-                                         None if counts is None else counts.data_ptr(), K.data_ptr(),
-                                         V.data_ptr(), _stream(dev))
-    _lib.check(rc)
+    _lib.check(_on_device(dev, _lib.load().asa_cache_write, cache._ref, ctypes.byref(t),
+                          None if counts is None else counts.data_ptr(), K.data_ptr(),
+                          V.data_ptr(), _stream(dev)))
 
 
 def read_tokens(cache, page_table, lengths, n=None, dtype=torch.bfloat16, start=None):
@@ -278,10 +283,8 @@ def read_tokens(cache, page_table, lengths, n=None, dtype=torch.bfloat16, start=
     V = torch.empty_like(K)
     t = _lib.CacheTokens(B, n, ops._DTYPES[dtype], table.size(1), table.data_ptr(),
                          None if start is None else start.data_ptr())
-    with ops._on_device(dev):
-        rc = _lib.load().asa_cache_read(cache._ref, ctypes.byref(t), lengths.data_ptr(),
-                                        K.data_ptr(), V.data_ptr(), _stream(dev))
-    _lib.check(rc)
+    _lib.check(_on_device(dev, _lib.load().asa_cache_read, cache._ref, ctypes.byref(t),
+                          lengths.data_ptr(), K.data_ptr(), V.data_ptr(), _stream(dev)))
     return K, V
 
 
@@ -339,16 +342,17 @@ def attend(cache, Q, page_table, lengths, Q_idx, alpha: float, sm_scale: float,
         a.q_strides[:] = qs
     ref = ctypes.byref(a)
     key = (B, H, NQ, dtype, P, most)
-    with ops._on_device(dev):
-        need = cache._workspaces.get(key)
-        if need is None:
-            z = ctypes.c_size_t()
-            _lib.check(lib.asa_cache_attention_workspace(cache._ref, ref, ctypes.byref(z)))
-            need = cache._workspaces[key] = z.value
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        rc = lib.asa_cache_attention(cache._ref, ref, Q.data_ptr(), out.data_ptr(),
-                                     None if ws is None else ws.data_ptr(), _stream(dev))
-    _lib.check(rc)
+    need = cache._workspaces.get(key)
+    if need is None:
+        if len(cache._workspaces) >= 1024:
+            cache._workspaces.clear()
+        z = ctypes.c_size_t()
+        _lib.check(_on_device(dev, lib.asa_cache_attention_workspace, cache._ref, ref,
+                              ctypes.byref(z)))
+        need = cache._workspaces[key] = z.value
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib.check(_on_device(dev, lib.asa_cache_attention, cache._ref, ref, Q.data_ptr(),
+                          out.data_ptr(), None if ws is None else ws.data_ptr(), _stream(dev)))
     return out
 
 
