@@ -252,21 +252,27 @@ struct KeyGranule {
       }
       whole = on;
     } else {
-      whole = true;
+      // a page for each tile (read without branches: positions past the last
+      // key take its page, and are not seen)
+      whole = base + kGranule <= key1;
+      int pg[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        pg[u] = __builtin_amdgcn_readfirstlane(pages[(min(base + kTile * u, key1 - 1) - key0) >> c.page_shift]);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int key = base + kTile * u;
-        const int pg = key < key1 ? __builtin_amdgcn_readfirstlane(pages[(key - key0) >> c.page_shift]) : -1;
-        whole = whole && pg >= 0;
-        const size_t row = (size_t(pg >= 0 ? pg : 0) * c.heads + h) * c.page + (key & (c.page - 1));
-        words<NG>(w[u], codes + row * (4 * NG) + col * (4 * NG) + NG * o);
+        whole = whole && pg[u] >= 0;
+        const size_t row = (size_t(pg[u] >= 0 ? pg[u] : 0) * c.heads + h) * c.page + ((base + kTile * u) & (c.page - 1));
+        words<NG>(w[u], codes + row * (4 * NG) + (col * (4 * NG) + NG * o));
       }
 #pragma unroll
       for (int v = 0; v < V; ++v) {
+        // the lane's own tile is P v + o P / 4
+        int mine = pg[P * v];
+        for (int u = 1; u < P; ++u) mine = o * P / 4 == u ? pg[P * v + u] : mine;
         const int key = base + kTile * (P * v + o * P / 4);
-        const int pg = key < key1 ? pages[(key - key0) >> c.page_shift] : -1;
-        seen[v] = pg >= 0;
-        const size_t row = (size_t(pg >= 0 ? pg : 0) * c.heads + h) * c.page + (key & (c.page - 1)) + col;
+        seen[v] = mine >= 0 && key < key1;
+        const size_t row = (size_t(mine >= 0 ? mine : 0) * c.heads + h) * c.page + (key & (c.page - 1)) + col;
         words<NG>(pr[v], c.k_params + row * NG);
       }
     }
