@@ -39,18 +39,23 @@ __device__ __forceinline__ void load8(const T* src, int nv, float* x) {
   }
 }
 
+// Values read back are stored past the caches: most of a read's bytes are its
+// results, and a batch of contexts is larger than the caches (8 x 8191, 268 MB
+// of results: 59.6 -> 44.9 us, 7.0 TB/s with the reads; a 16k prompt written
+// and read 39.7 -> 32.7; 17 MB unchanged).
 template <typename T, bool CHUNKS>
 __device__ __forceinline__ void store8(T* dst, int nv, const float* x) {
   if constexpr (CHUNKS) {
     if constexpr (std::is_same<T, float>::value) {
-      *reinterpret_cast<float4*>(dst) = float4{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<float4*>(dst + 4) = float4{x[4], x[5], x[6], x[7]};
+      __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4*>(dst));
+      __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4*>(dst + 4));
     } else {
+      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
       T e[8];
       for (int j = 0; j < 8; ++j) Elem<T>::store(e + j, x[j]);
-      uint4 u;
+      u32x4 u;
       __builtin_memcpy(&u, e, 16);
-      *reinterpret_cast<uint4*>(dst) = u;
+      __builtin_nontemporal_store(u, reinterpret_cast<u32x4*>(dst));
     }
   } else {
     for (int j = 0; j < 8; ++j)
