@@ -23,8 +23,8 @@
 // tiles share the 16 rows of one result: tile u's operand holds the queries
 // in rows u (16 / P) .. and zeros elsewhere, so that its products add to
 // those of the other tiles without meeting them, and each lane of the result
-// has a key of its own to scale (about 280 vector instructions per 64 keys of
-// head dimension 128 at P = 4, 600 before).
+// has a key of its own to scale (about 250 vector instructions per 64 keys of
+// head dimension 128 at P = 4).
 //
 // tau lies in [max z - 1, max z], so only keys with z > max z - 1 can have a
 // weight.  A better bound: the sum over any part of the row is at most the
@@ -125,7 +125,7 @@ struct QueryLds {
   static constexpr int kR = kTile / P;
   static constexpr int NT = std::is_same<T, float>::value ? 3 : 1;
   uint4 a[NG][NT][4 * kR + 1];  // [..][octet * kR + row], zeros
-  alignas(16) float bias[NG][kTile];  // -16 sum q_g of each row
+  f32x4 bias[NG][kTile / 4];        // -16 sum q_g of each row
 };
 
 // 8 channels of a query row from `ch` on, zeros past the head dimension.
@@ -164,7 +164,7 @@ __device__ __forceinline__ void stage_query(const CacheAttnParams& p, QueryLds<T
     load_query<T>(p, q, 32 * g + 8 * o, x);
     for (int j = 0; j < 8; ++j) x[j] = ok ? x[j] * sign : 0.0f;
     const float sum = sum_groups(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
-    if (o == 0) ql.bias[g][r] = -16.0f * sum;
+    if (o == 0) reinterpret_cast<float*>(ql.bias[g])[r] = -16.0f * sum;
 #pragma unroll
     for (int t = 0; t < QL::NT; ++t) {
       CodeVec<T> v;
@@ -197,7 +197,7 @@ struct TileRows {
   __device__ __forceinline__ void load(const CacheAttnParams& p, int b, int r0, int lane) {
     const int o = lane >> 4, ar = lane & 15, row = r0 + ar % kR;
     for (int u = 0; u < P; ++u) at[u] = ar / kR == u ? o * kR + ar % kR : 4 * kR;
-    bias = (4 * o) % kR;
+    bias = o % (kR / 4);
     const int v = row < p.R ? visible_keys(p, b, row % p.NQ) : 0;
     most = wave_reduce_minmax<true>(v);
     least = wave_reduce_minmax<false>(row < p.R ? v : INT_MAX);
@@ -289,7 +289,7 @@ __device__ __forceinline__ void dots(const QueryLds<T, P, NG>& ql, const TileRow
   for (int v = 0; v < V; ++v) s[v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    const f32x4 bias = *reinterpret_cast<const f32x4*>(&ql.bias[g][t.bias]);
+    const f32x4 bias = ql.bias[g][t.bias];
     CodeVec<T> a[P][NT];
 #pragma unroll
     for (int u = 0; u < P; ++u)
