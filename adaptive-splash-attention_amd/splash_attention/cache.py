@@ -192,12 +192,36 @@ class QuantizedKVCache:
         K, V: [B, kv_heads, n, head_dim] of one type (float32, bfloat16 or
         float16), with any strides (read in place where the channels are next
         to each other).  start, counts: [B] integers.  Every other row stays
-        as it is.  Two tokens of one call must not share a row: sequences that
-        share pages write to them in different calls."""
+        as it is.  Two tokens of one call must not share a row (which of the
+        two rows' bytes stay is not defined): sequences that share pages write
+        to them in different calls.  check_write tells."""
         if torch.compiler.is_compiling():
             from . import library
             return library.cache_write(self, K, V, page_table, start, counts)
         write_tokens(self, K, V, page_table, start, counts)
+
+    def check_write(self, page_table, start, n: int, counts=None) -> None:
+        """Debug check (synchronises): raises ValueError if a write of n
+        tokens per sequence with these arguments had a token without a row,
+        or two tokens with the same one."""
+        dev = self.device
+        table = _table(page_table, None, dev).long()
+        B, P = table.shape
+        start = _i32(start, (B,), dev, "start").long()
+        i = torch.arange(int(n), device=dev)
+        live = torch.ones((B, int(n)), dtype=torch.bool, device=dev)
+        if counts is not None:
+            live = i < _i32(counts, (B,), dev, "counts")[:, None]
+        at = start[:, None] + i
+        col = at // self.page_size
+        page = table.gather(1, col.clamp(0, P - 1))
+        fine = (at >= 0) & (col < P) & (page >= 0) & (page < self.num_pages)
+        if bool((live & ~fine).any()):
+            raise ValueError("a token has no row: its position is negative or past the page "
+                             "table, or its entry is not a page of the cache")
+        rows = (page * self.page_size + at % self.page_size)[live]
+        if rows.unique().numel() != rows.numel():
+            raise ValueError("two tokens go to the same row")
 
     def read(self, page_table, lengths, n: int | None = None, dtype=torch.bfloat16, start=None):
         """The cached keys and values (K, V), [B, kv_heads, n, head_dim], of

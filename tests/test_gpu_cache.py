@@ -286,7 +286,7 @@ def test_attention_over_alphas(dev, alpha, n):
     check_attention(out, q, k, v, [n], [[n - 1]], alpha, 0.125, f"alpha {alpha}")
 
 
-@pytest.mark.parametrize("n,qscale", [(1500, 1e-4), (1500, 0.0), (12000, 1e-4), (12000, 0.0), (20000, 0.05), (2000, 40.0)])
+@pytest.mark.parametrize("n,qscale", [(900, 1e-4), (900, 0.0), (900, 0.1), (1500, 1e-4), (1500, 0.0), (12000, 1e-4), (12000, 0.0), (20000, 0.05), (2000, 40.0)])
 @pytest.mark.parametrize("alpha", [1.5, 2.0, 1.25, 2.5])
 def test_flat_and_peaked_rows(dev, n, qscale, alpha):
     """Near-uniform rows, whose candidates fit no list, rows with every score
@@ -476,6 +476,37 @@ def test_many_tiles_in_one_launch(dev, HK, rep, n):
     for h in (0, HK - 1):
         check_attention(out[:, h * rep:(h + 1) * rep], q[:, h * rep:(h + 1) * rep], k[:, h:h + 1], v[:, h:h + 1],
                         [n, n - 70], default_idx([n, n - 70], 1), 1.5, d ** -0.5)
+
+
+@pytest.mark.parametrize("alpha", [1.5, 1.25])
+@pytest.mark.parametrize("rep,qscale", [(16, 1e-3), (16, 0.3), (5, 0.0), (1, 1e-3)])
+def test_flat_rows_of_many_tiles(dev, rep, qscale, alpha):
+    """Rows whose candidates fit no list, several to a block, some blocks with
+    more rows than waves."""
+    HK, n, d = 100, 900, 32
+    c, table, L, k, v = filled(dev, [n, 650], HK, d, 64, torch.float32, 24)
+    q = torch.randn(2, HK * rep, 1, d, generator=torch.Generator().manual_seed(9)) * qscale
+    out = c.attention(q.to(dev), table, L, alpha=alpha)
+    for h in (0, 57):
+        check_attention(out[:, h * rep:(h + 1) * rep], q[:, h * rep:(h + 1) * rep], k[:, h:h + 1], v[:, h:h + 1],
+                        [n, 650], default_idx([n, 650], 1), alpha, d ** -0.5)
+
+
+def test_check_write(dev):
+    """The debug check: every token of a write has a row, and its own."""
+    c = make(dev, 4, 1, 32, 16)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    c.check_write(t([[0, 1], [2, 3]]), t([0, 5]), 20)
+    c.check_write(t([[0, 1], [0, 3]]), t([0, 16]), 16)           # a shared page, one writer
+    c.check_write(t([[0, 1], [0, -1]]), t([0, 0]), 20, t([20, 0]))
+    with pytest.raises(ValueError, match="same row"):
+        c.check_write(t([[0, 1], [0, 3]]), t([0, 10]), 16)
+    with pytest.raises(ValueError, match="no row"):
+        c.check_write(t([[0, 1], [2, 4]]), t([0, 0]), 20)
+    with pytest.raises(ValueError, match="no row"):
+        c.check_write(t([[0, 1]]), t([30]), 3)
+    with pytest.raises(ValueError, match="no row"):
+        c.check_write(t([[0, 1]]), t([-1]), 3)
 
 
 def test_two_threads_call_at_once(dev):
