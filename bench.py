@@ -57,8 +57,8 @@ COPY_BYTES = 256 << 20   # --copy-calibration copy size
 # library built from the sources whose hash is HBM_TRAFFIC_SOURCES
 # (source_hash()).  A line from a library built from other sources reports
 # traffic null and says why: counters of another build are not evidence.
-HBM_TRAFFIC_SOURCES = "29048bb7d45382c7"
-HBM_TRAFFIC = {'bounds': 1110674, 'select': 141539022, 'tau': 34740416, 'tau_compact': 37521280, 'refine': 109852944, 'compact': 2761045, 'forward': 330553433, 'bwd_dq_sparse': 240731648, 'bwd_dkdv_sparse': 287763040}
+HBM_TRAFFIC_SOURCES = "9c27ce0028500079"
+HBM_TRAFFIC = {'bounds': 1109820, 'select': 141478756, 'tau': 34740395, 'tau_compact': 37524075, 'refine': 109676421, 'compact': 2761045, 'forward': 330253099, 'bwd_dq_sparse': 240753716, 'bwd_dkdv_sparse': 287762512}
 
 
 def source_hash() -> str:
